@@ -1,0 +1,245 @@
+"""The 8-bit feed-forward operators of the library: what serving and adapter training call them for, from one decoded token to an
+8192-row prefill, and their plain forms.
+
+Five operators, on int8 weights [N, K] with one fp32 scale a row (output channel) and activations with one scale a row (token):
+  quantize     float rows -> int8 codes and scales
+  matmul       y = x @ w^T, x float (quantized within the call) or int8 codes with their scales; with or without a bias
+  gate_up      y = silu(x @ wg^T) * (x @ wu^T); a training step keeps both projections for the backward pass
+  matmul_bwd   the gradient of matmul to its activations
+  gate_up_bwd  the gradients of gate_up to its activations and to both projections
+"""
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+def quantize(M, K, dtype="bf16"):
+    return {"op": "quantize", "M": M, "K": K, "dtype": dtype}
+
+
+def matmul(M, N, K, dtype="bf16", codes=False, bias=False):
+    """codes: x comes as int8 codes with their scales (several layers read the same tokens)."""
+    return {"op": "matmul", "M": M, "N": N, "K": K, "dtype": dtype, "codes": codes, "bias": bias}
+
+
+def gate_up(M, N, K, dtype="bf16", codes=False, save=False):
+    return {"op": "gate_up", "M": M, "N": N, "K": K, "dtype": dtype, "codes": codes, "save": save}
+
+
+def matmul_bwd(M, N, K, dtype="bf16"):
+    return {"op": "matmul_bwd", "M": M, "N": N, "K": K, "dtype": dtype}
+
+
+def gate_up_bwd(M, N, K, dtype="bf16"):
+    return {"op": "gate_up_bwd", "M": M, "N": N, "K": K, "dtype": dtype}
+
+
+def listed():
+    return [
+        # the activations of one decoded token, ahead of layers that share them: latency
+        dict(quantize(1, 4096), name="quantize_m1"),
+        # the widest activations of a long prompt, ahead of the down projections
+        dict(quantize(8192, 14336), name="quantize_m8192"),
+        # one attention projection of one decoded token: latency and the weight's bytes
+        dict(matmul(1, 4096, 4096), name="matmul_m1"),
+        # a short prompt through a projection of no round size, fp16, with a bias
+        dict(matmul(77, 1111, 2000, dtype="fp16", bias=True), name="matmul_m77_ragged_fp16"),
+        # the largest product: a long prompt through the down projection of an 8B model
+        dict(matmul(8192, 4096, 14336, codes=True), name="matmul_m8192"),
+        # the feed-forward input of one decoded token of an 8B model
+        dict(gate_up(1, 14336, 4096), name="gate_up_m1"),
+        # a decode batch through the same block, the tokens quantized before
+        dict(gate_up(48, 14336, 4096, codes=True), name="gate_up_m48"),
+        # a training batch of no round length, both projections kept
+        dict(gate_up(2003, 14336, 4096, save=True), name="gate_up_m2003_save"),
+        # the gradient through the down projection of a training batch
+        dict(matmul_bwd(2048, 4096, 14336), name="matmul_bwd_m2048"),
+        # a small layer's gradient in fp32
+        dict(matmul_bwd(300, 1536, 2048, dtype="fp32"), name="matmul_bwd_m300_fp32"),
+        # the gradient through the feed-forward input of a training batch
+        dict(gate_up_bwd(4096, 14336, 4096), name="gate_up_bwd_m4096"),
+        # a small model's, a short sequence in fp16
+        dict(gate_up_bwd(77, 5632, 2048, dtype="fp16"), name="gate_up_bwd_m77_fp16"),
+    ]
+
+
+# (N, K) of projections, and (inter, hidden) of feed-forward blocks
+SHAPES = [(4096, 4096), (14336, 4096), (4096, 14336), (1024, 4096), (2048, 7168), (7168, 2048), (1536, 2048), (2048, 768)]
+BLOCKS = [(14336, 4096), (2048, 7168), (768, 2048), (5632, 2048)]
+
+
+def _log_int(rng, lo, hi):
+    return min(hi, int(math.exp(rng.uniform(math.log(lo), math.log(hi + 1)))))
+
+
+def draw(rng):
+    op = rng.choice(("quantize", "matmul", "matmul", "gate_up", "gate_up", "matmul_bwd", "gate_up_bwd"))
+    dtype = rng.choice(("bf16", "bf16", "bf16", "fp16", "fp32"))
+    if op == "quantize":
+        return quantize(_log_int(rng, 1, 8192), _log_int(rng, 64, 14336), dtype)
+    top = {"matmul": 8192, "gate_up": 4096, "matmul_bwd": 4096, "gate_up_bwd": 2500 if dtype == "bf16" else 1200}[op]
+    M = _log_int(rng, 1, top)
+    r = rng.random()
+    if r < 0.6:
+        N, K = rng.choice(SHAPES if op.startswith("matmul") else BLOCKS)
+    elif r < 0.9:  # widths off the usual multiples
+        N, K = _log_int(rng, 33, 8192), 16 * _log_int(rng, 4, 512)
+    else:  # any size at all
+        N, K = _log_int(rng, 1, 4096), _log_int(rng, 1, 4096)
+    if op == "matmul":
+        return matmul(M, N, K, dtype, codes=rng.random() < 0.4, bias=rng.random() < 0.3)
+    if op == "gate_up":
+        return gate_up(M, N, K, dtype, codes=rng.random() < 0.4, save=rng.random() < 0.4)
+    return matmul_bwd(M, N, K, dtype) if op == "matmul_bwd" else gate_up_bwd(M, N, K, dtype)
+
+
+def _activations(g, M, K, dtype):
+    """Normal values with a few channels ten to thirty times larger, as the hidden states of language models have them."""
+    x = torch.randn(M, K, device="cuda", generator=g)
+    big = torch.rand(K, device="cuda", generator=g)
+    return (x * torch.where(big < 0.005, 10 + 4000 * big, torch.ones_like(big))).to(dtype)
+
+
+def _weights(g, N, K):
+    w = torch.randn(N, K, device="cuda", generator=g) * 0.02
+    s = w.abs().amax(1) / 127
+    return torch.clamp(torch.round(w / s[:, None]), -127, 127).to(torch.int8), s
+
+
+def prepare(case, seed):
+    g = torch.Generator(device="cuda").manual_seed(int(seed))
+    c, dtype = case, DTYPES[case["dtype"]]
+    st = {"case": dict(case), "dtype": dtype}
+    if c["op"] == "quantize":
+        st["x"] = _activations(g, c["M"], c["K"], dtype)
+        return st
+    st["w"], st["s"] = _weights(g, c["N"], c["K"])
+    if c["op"].startswith("gate_up"):
+        st["wu"], st["su"] = _weights(g, c["N"], c["K"])
+    if c["op"] in ("matmul", "gate_up"):
+        st["x"], st["sx"] = _activations(g, c["M"], c["K"], dtype), None
+        if c["codes"]:
+            st["x"], st["sx"] = _codes(st["x"])
+        st["bias"] = torch.randn(c["N"], device="cuda", generator=g).to(dtype) if c.get("bias") else None
+        return st
+    # gradients of a mean over the tokens: small numbers
+    st["dy"] = (torch.randn(c["M"], c["N"], device="cuda", generator=g) * 2e-3).to(dtype)
+    if c["op"] == "gate_up_bwd":
+        st["gate"] = torch.randn(c["M"], c["N"], device="cuda", generator=g).to(dtype)
+        st["up"] = torch.randn(c["M"], c["N"], device="cuda", generator=g).to(dtype)
+    return st
+
+
+def _codes(x):
+    """Codes and scales of float rows. The quotient is taken in 64 bits: codes are the nearest integers to x / s, and some x lie
+    next to the border between two."""
+    s = (x.float().abs().amax(-1).double() / 127).float()
+    q = torch.round(x.double() / s.double()[:, None]).nan_to_num(0.0)
+    return torch.clamp(q, -127, 127).to(torch.int8), s
+
+
+def _product(x, sx, w, s):
+    return (x.float() @ w.float().t()) * sx[:, None] * s[None, :]
+
+
+def run(st):
+    op = st["case"]["op"]
+    if own:
+        mi = _library()
+        if op == "quantize":
+            return mi.int8_quantize(st["x"])
+        if op == "matmul":
+            return mi.int8_matmul(st["x"], st["w"], st["s"], x_scales=st["sx"], bias=st["bias"], dtype=st["dtype"])
+        if op == "gate_up":
+            return mi.int8_gate_up_swiglu(st["x"], st["w"], st["s"], st["wu"], st["su"], x_scales=st["sx"], dtype=st["dtype"],
+                                          save=st["case"]["save"])
+        if op == "matmul_bwd":
+            return mi.int8_matmul_backward(st["dy"], st["w"], st["s"])
+        return mi.int8_gate_up_swiglu_backward(st["dy"], st["gate"], st["up"], st["w"], st["s"], st["wu"], st["su"])
+    dtype = st["dtype"]
+    if op == "quantize":
+        return _codes(st["x"])
+    if op in ("matmul", "gate_up"):
+        x, sx = (st["x"], st["sx"]) if st["sx"] is not None else _codes(st["x"])
+        y = _product(x, sx, st["w"], st["s"])
+        if op == "matmul":
+            return (y if st["bias"] is None else y + st["bias"].float()).to(dtype)
+        u = _product(x, sx, st["wu"], st["su"])
+        h = (y / (1 + torch.exp(-y)) * u).to(dtype)
+        return (h, y.to(dtype), u.to(dtype)) if st["case"]["save"] else h
+    dy = st["dy"].float()
+    if op == "matmul_bwd":
+        return ((dy * st["s"]) @ st["w"].float()).to(dtype)
+    g, u = st["gate"].float(), st["up"].float()
+    sig = 1 / (1 + torch.exp(-g))
+    dg, du = dy * u * sig * (1 + g * (1 - sig)), dy * g * sig
+    dx = (dg * st["s"]) @ st["w"].float() + (du * st["su"]) @ st["wu"].float()
+    return dx.to(dtype), dg.to(dtype), du.to(dtype)
+
+
+def _library():
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "mlx-serve_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    import mi_qmm
+    return mi_qmm
+
+
+def work(case):
+    c, e = case, 4 if case["dtype"] == "fp32" else 2
+    M, K = c["M"], c["K"]
+    if c["op"] == "quantize":
+        return {"bytes": M * K * (e + 1) + 4 * M, "flops": 3 * M * K}
+    N = c["N"]
+    x = M * K + 4 * M if c.get("codes") else M * K * e
+    if c["op"] == "matmul":
+        return {"bytes": N * K + 4 * N + x + M * N * e + (N * e if c["bias"] else 0), "flops": 2 * M * N * K}
+    if c["op"] == "gate_up":
+        return {"bytes": 2 * (N * K + 4 * N) + x + M * N * e * (3 if c["save"] else 1), "flops": 4 * M * N * K}
+    if c["op"] == "matmul_bwd":
+        return {"bytes": N * K + 4 * N + M * N * e + M * K * e, "flops": 2 * M * N * K}
+    return {"bytes": 2 * (N * K + 4 * N) + 5 * M * N * e + M * K * e, "flops": 4 * M * N * K}
+
+
+def _exact_codes(x):
+    """(codes, fp32 scales): the integer part of |x| / s, one more above a half and, on a half, where it is odd."""
+    a = x.double().abs()
+    s = (a.max(dim=1).values / 127.0).to(torch.float32)
+    r = a / s.double().unsqueeze(1)
+    n = r.floor()
+    n = n + ((r - n > 0.5) | ((r - n == 0.5) & (n % 2 == 1))).double()
+    n = torch.where(torch.isnan(n), torch.zeros_like(n), n.clamp(max=127.0))
+    return torch.where(x.double() < 0, -n, n), s
+
+
+def exact(case, seed):
+    st = prepare(case, seed)
+    op = case["op"]
+    if op == "quantize":
+        q, s = _exact_codes(st["x"])
+        return q.to(torch.int8), s.double()
+    w = st["w"].double() * st["s"].double().unsqueeze(1)
+    wu = st["wu"].double() * st["su"].double().unsqueeze(1) if "wu" in st else None
+    if op in ("matmul", "gate_up"):
+        q, s = _exact_codes(st["x"]) if st["sx"] is None else (st["x"].double(), st["sx"])
+        x = q * s.double().unsqueeze(1)
+        y = torch.matmul(x, w.T)
+        if op == "matmul":
+            return y if st["bias"] is None else torch.add(y, st["bias"].double())
+        u = torch.matmul(x, wu.T)
+        h = torch.mul(torch.mul(y, torch.special.expit(y)), u)
+        return (h, y, u) if case["save"] else h
+    dy = st["dy"].double()
+    if op == "matmul_bwd":
+        return torch.matmul(dy, w)
+    g, u = st["gate"].double(), st["up"].double()
+    s = torch.special.expit(g)
+    # d/dg of g s(g): s + g s (1 - s)
+    dg, du = dy * u * (s + g * s * (1 - s)), dy * (g * s)
+    return torch.matmul(dg, w) + torch.matmul(du, wu), dg, du
