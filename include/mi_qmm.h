@@ -41,6 +41,7 @@ enum {
 enum {
   MI_DTYPE_UINT8 = 1,
   MI_DTYPE_UINT32 = 3,
+  MI_DTYPE_INT8 = 5,
   MI_DTYPE_FLOAT16 = 9,
   MI_DTYPE_FLOAT32 = 10,
   MI_DTYPE_BFLOAT16 = 12,
@@ -276,6 +277,71 @@ int mi_gather_qmv_down_reduce(void* y, const void* act, const uint32_t* w_down,
                               const void* scores, int64_t T, int k, int64_t N, int64_t K,
                               int64_t n_experts, mi_optional_int group_size, mi_optional_int bits,
                               const char* mode, void* stream);
+
+/* ------------------------------------------------- int8 weights and activations ---
+ * A feed-forward block (or any linear layer) on the int8 matrix cores: int8 weights [N, K] with
+ * one fp32 scale a row (output channel), activations [M, K] with one scale a row (token). No
+ * counterpart in the reference, whose quantized layers are weight-only; an affine checkpoint's
+ * layer becomes one by mi_int8_quantize(mi_dequantize(w)), row by row.
+ *
+ * x comes as int8 codes (x_dtype int8) with x_scales [M], or as floats (x_dtype bfloat16,
+ * float16 or float32, x_scales NULL), which the call quantizes first: bit-equal to
+ * mi_int8_quantize before it, and the way to go for one layer. y is bfloat16, float16 or float32.
+ *
+ * Workspace: device memory of the caller's, aligned to 16 bytes, that no other call uses until
+ * this one has run; its size comes from the two functions below (host only; may be 0, then
+ * NULL will do; -1 for sizes or types out of range). A missing or short one is
+ * MI_ERR_WORKSPACE. These calls allocate nothing and keep nothing, so they can be captured into
+ * graphs as they are, and run at the same time on several streams with a workspace each.
+ * Outputs must not overlap inputs. Empty outputs (M = 0, ...) are no-ops; a sum over nothing
+ * (K = 0 forward, N = 0 backward) is MI_ERR_INVALID. K over 131071 forward, where the int32 sums
+ * of the products could overflow, is MI_ERR_UNSUPPORTED. */
+
+/* scales[r] = max_k |x[r,k]| / 127 (one rounding to fp32); q[r,k] the integer nearest to
+ * x[r,k] / scales[r], ties to even. A zero row has scale 0 and codes 0. A row that holds an
+ * infinity or a NaN has that as its scale and codes 0, so that its products are NaN.
+ * q [rows, K], scales [rows]; x bfloat16, float16 or float32. For weights and activations alike. */
+int mi_int8_quantize(int8_t* q, float* scales, const void* x, int64_t rows, int64_t K, int x_dtype,
+                     void* stream);
+
+/* Workspace bytes of the calls below; banks: 1 for the product, 2 for gate + up. */
+int64_t mi_int8_forward_workspace(int64_t M, int64_t N, int64_t K, int banks, int x_dtype);
+int64_t mi_int8_backward_workspace(int64_t M, int64_t N, int64_t K, int banks, int dtype);
+
+/* y[m,n] = x_scales[m] * w_scales[n] * sum_k x[m,k] w[n,k] (+ bias[n]): int32 sums, exact, the
+ * scales and the bias in fp32, one rounding to y_dtype. bias: NULL, or [N] in y's type. */
+int mi_int8_matmul(void* y, const void* x, const float* x_scales, const int8_t* w,
+                   const float* w_scales, const void* bias, int64_t M, int64_t N, int64_t K,
+                   int x_dtype, int y_dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* y = silu(g) * u with g and u the products of x with w_gate and w_up (as mi_int8_matmul),
+ * silu(g) = g / (1 + e^-g) in fp32, one rounding. gate and up: both NULL, or [M, N] in y's type
+ * for g and u, each rounded once, as the backward pass takes them. */
+int mi_int8_gate_up_swiglu(void* y, void* gate, void* up, const void* x, const float* x_scales,
+                           const int8_t* w_gate, const float* s_gate, const int8_t* w_up,
+                           const float* s_up, int64_t M, int64_t N, int64_t K, int x_dtype,
+                           int y_dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The gradient of mi_int8_matmul to its activations: dx[m,k] = sum_n dy[m,n] w_scales[n] w[n,k].
+ * Weights and scales are constants (a frozen base under adapters), and the rounding of the
+ * activations is passed straight through. dy [M, N] and dx [M, K] in dtype (bfloat16, float16 or
+ * float32), fp32 sums. For bfloat16 each dy * scale is rounded once to bfloat16; for
+ * float16 / float32 it keeps 16 / 24 bits. */
+int mi_int8_matmul_backward(void* dx, const void* dy, const int8_t* w, const float* w_scales,
+                            int64_t M, int64_t N, int64_t K, int dtype, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+
+/* The gradients of mi_int8_gate_up_swiglu: with s = 1 / (1 + e^-g),
+ *   dgate = dy * u * s * (1 + g (1 - s)),   dup = dy * g * s   (fp32, one rounding each)
+ *   dx[m,k] = sum_n dgate[m,n] s_gate[n] w_gate[n,k] + dup[m,n] s_up[n] w_up[n,k]
+ * from gate and up as the forward call gave them; dx is formed from dgate and dup before their
+ * rounding, otherwise as mi_int8_matmul_backward. dgate and dup ([M, N], both or neither NULL)
+ * are what adapters on either projection, and the gradients of the channel scales, start from. */
+int mi_int8_gate_up_swiglu_backward(void* dx, void* dgate, void* dup, const void* dy,
+                                    const void* gate, const void* up, const int8_t* w_gate,
+                                    const float* s_gate, const int8_t* w_up, const float* s_up,
+                                    int64_t M, int64_t N, int64_t K, int dtype, void* workspace,
+                                    int64_t workspace_bytes, void* stream);
 
 /* Grow the per-device workspace (sorted work lists, K-split partials) to at least
  * `bytes` ahead of HIP graph capture; calls that fit never allocate. No mlx-c

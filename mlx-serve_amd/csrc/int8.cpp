@@ -1,0 +1,216 @@
+// C ABI of the int8 operators (include/mi_qmm.h): validation, dispatch, workspace layout. The
+// workspace belongs to the caller, so calls on different streams and graphs share nothing.
+#include <string>
+
+#include "int8.h"
+#include "mi_qmm.h"
+
+namespace mi {
+int report_error(int code, const std::string& msg);  // sets mi_last_error() (api.cpp)
+}
+
+namespace {
+
+using mi::report_error;
+
+constexpr int64_t kMaxDim = (int64_t)1 << 30;
+constexpr int64_t kMaxTiles = (int64_t)1 << 22;  // blocks of up to 512 threads: below 2^32 threads
+constexpr int64_t kMaxArea = (int64_t)1 << 40;   // values of a gradient
+
+int bad(const char* msg) { return report_error(MI_ERR_INVALID, msg); }
+int hip_status(hipError_t e, const char* what) {
+  return e == hipSuccess ? MI_OK
+                         : report_error(MI_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
+}
+
+int float_type(int dtype) {
+  return dtype == MI_DTYPE_BFLOAT16  ? mi::kBF16
+         : dtype == MI_DTYPE_FLOAT16 ? mi::kF16
+         : dtype == MI_DTYPE_FLOAT32 ? mi::kF32
+                                     : -1;
+}
+
+int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// Shared by the five calls: sizes and the workspace the caller gave. `need` 0: none is used.
+int check_sizes(int64_t M, int64_t N, int64_t K) {
+  if (M < 0 || N < 0 || K < 0) return bad("negative size");
+  if (M > kMaxDim || N > kMaxDim || K > kMaxDim) return bad("M, N or K too large");
+  return MI_OK;
+}
+int check_workspace(const void* ws, int64_t given, int64_t need) {
+  if (need == 0) return MI_OK;
+  if (!ws || given < need)
+    return report_error(MI_ERR_WORKSPACE, "this call needs a workspace of " + std::to_string(need) +
+                                              " bytes, " + std::to_string(ws ? given : 0) + " given");
+  if ((uintptr_t)ws % 16) return bad("the workspace must be aligned to 16 bytes");
+  return MI_OK;
+}
+
+// Forward workspace: codes [M, ldx], then scales, of activations that come as floats.
+int64_t codes_bytes(int64_t M, int64_t K) { return up(M * up(K, 16), 256); }
+int64_t forward_need(int64_t M, int64_t K, int x_dtype) {
+  if (x_dtype == MI_DTYPE_INT8 || M == 0) return 0;
+  return codes_bytes(M, K) + M * 4;
+}
+
+int forward(mi::Int8Params& P, const void* x, const float* x_scales, int64_t M, int64_t N,
+            int64_t K, int x_dtype, int y_dtype, void* ws, int64_t ws_bytes, hipStream_t s) {
+  if (int rc = check_sizes(M, N, K)) return rc;
+  if (K == 0) return bad("K must be positive");
+  P.type = float_type(y_dtype);
+  if (P.type < 0) return report_error(MI_ERR_UNSUPPORTED, "y dtype not supported (bfloat16, float16, float32)");
+  const int xt = float_type(x_dtype);
+  if (xt < 0 && x_dtype != MI_DTYPE_INT8)
+    return report_error(MI_ERR_UNSUPPORTED, "x dtype not supported (int8, bfloat16, float16, float32)");
+  if (K > mi::kInt8MaxK)
+    return report_error(MI_ERR_UNSUPPORTED, "K over 131071: the int32 sums could overflow");
+  if (xt >= 0 && x_scales) return bad("x_scales belong to int8 x");
+  if (M == 0 || N == 0) return MI_OK;
+  if (((M + 63) / 64) * ((N + 63) / 64) > kMaxTiles)
+    return report_error(MI_ERR_UNSUPPORTED, "M * N too large for one call");
+  if (!P.y || !x || !P.w || !P.sw || (xt < 0 && !x_scales)) return bad("null tensor pointer");
+  if (int rc = check_workspace(ws, ws_bytes, forward_need(M, K, x_dtype))) return rc;
+  P.M = (int)M;
+  P.N = (int)N;
+  P.K = (int)K;
+  P.x = (const int8_t*)x;
+  P.sx = x_scales;
+  P.ldx = K;
+  if (xt >= 0) {
+    P.ldx = up(K, 16);
+    P.x = (const int8_t*)ws;
+    P.sx = (const float*)((char*)ws + codes_bytes(M, K));
+    const hipError_t e = mi::launch_int8_quantize((int8_t*)ws, (float*)P.sx, x, M, K, P.ldx, xt, s);
+    if (e != hipSuccess) return hip_status(e, "int8 quantize launch");
+  }
+  return hip_status(mi::launch_int8_any(P, s), "int8 matmul launch");
+}
+
+// Backward workspace: the bf16 parts of the incoming gradient, [banks * terms][M][np].
+int64_t np_of(int64_t N) { return up(N, 64); }
+int64_t backward_need(int64_t M, int64_t N, int banks, int type) {
+  return up(banks * (type + 1) * M * np_of(N) * 2, 256);
+}
+
+int backward(mi::Int8GradParams& G, mi::Int8BwdParams& B, int64_t M, int64_t N, int64_t K, int dtype,
+             int banks, void* ws, int64_t ws_bytes, hipStream_t s) {
+  if (int rc = check_sizes(M, N, K)) return rc;
+  if (N == 0) return bad("N must be positive");
+  const int type = float_type(dtype);
+  if (type < 0) return report_error(MI_ERR_UNSUPPORTED, "dtype not supported (bfloat16, float16, float32)");
+  if (M == 0 || K == 0) return MI_OK;
+  if (((M + 63) / 64) * ((K + 63) / 64) > kMaxTiles || M * N > kMaxArea)
+    return report_error(MI_ERR_UNSUPPORTED, "M * K or M * N too large for one call");
+  if (!G.dy || !G.sw || !B.dx || !B.w[0] || (banks == 2 && (!G.gate || !G.up || !G.sw2 || !B.w[1])))
+    return bad("null tensor pointer");
+  if (!G.dgate != !G.dup) return bad("dgate and dup go together");
+  if (int rc = check_workspace(ws, ws_bytes, backward_need(M, N, banks, type))) return rc;
+  G.a = (uint16_t*)ws;
+  G.banks = B.banks = banks;
+  G.terms = B.terms = type + 1;
+  G.np = B.np = (int)np_of(N);
+  G.M = B.M = (int)M;
+  G.N = B.N = (int)N;
+  B.K = (int)K;
+  G.type = B.type = type;
+  B.a = G.a;
+  B.splits = 1;
+  const hipError_t e = mi::launch_int8_grad(G, s);
+  if (e != hipSuccess) return hip_status(e, "int8 gradient launch");
+  return hip_status(mi::launch_int8_bwd_any(B, s), "int8 backward launch");
+}
+
+}  // namespace
+
+extern "C" {
+
+int mi_int8_quantize(int8_t* q, float* scales, const void* x, int64_t rows, int64_t K, int x_dtype,
+                     void* stream) {
+  if (int rc = check_sizes(0, 0, K)) return rc;
+  if (rows < 0) return bad("negative size");
+  const int type = float_type(x_dtype);
+  if (type < 0) return report_error(MI_ERR_UNSUPPORTED, "x dtype not supported (bfloat16, float16, float32)");
+  if (K == 0) return bad("K must be positive");
+  if (rows == 0) return MI_OK;
+  if (!q || !scales || !x) return bad("null tensor pointer");
+  return hip_status(mi::launch_int8_quantize(q, scales, x, rows, K, K, type, (hipStream_t)stream),
+                    "int8 quantize launch");
+}
+
+int64_t mi_int8_forward_workspace(int64_t M, int64_t N, int64_t K, int banks, int x_dtype) {
+  if (M < 0 || N < 0 || K < 0 || banks < 1 || banks > 2 || M > kMaxDim || K > kMaxDim) return -1;
+  return forward_need(M, K, x_dtype);
+}
+
+int64_t mi_int8_backward_workspace(int64_t M, int64_t N, int64_t K, int banks, int dtype) {
+  const int type = float_type(dtype);
+  if (M < 0 || N < 0 || K < 0 || banks < 1 || banks > 2 || type < 0 || M > kMaxDim || N > kMaxDim ||
+      M * N > kMaxArea)
+    return -1;
+  return backward_need(M, N, banks, type);
+}
+
+int mi_int8_matmul(void* y, const void* x, const float* x_scales, const int8_t* w,
+                   const float* w_scales, const void* bias, int64_t M, int64_t N, int64_t K,
+                   int x_dtype, int y_dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  mi::Int8Params P{};
+  P.y = y;
+  P.w = w;
+  P.sw = w_scales;
+  P.bias = bias;
+  return forward(P, x, x_scales, M, N, K, x_dtype, y_dtype, workspace, workspace_bytes,
+                 (hipStream_t)stream);
+}
+
+int mi_int8_gate_up_swiglu(void* y, void* gate, void* up, const void* x, const float* x_scales,
+                           const int8_t* w_gate, const float* s_gate, const int8_t* w_up,
+                           const float* s_up, int64_t M, int64_t N, int64_t K, int x_dtype,
+                           int y_dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (!gate != !up) return bad("gate and up go together");
+  if (M > 0 && N > 0 && (!w_up || !s_up)) return bad("null tensor pointer");
+  mi::Int8Params P{};
+  P.y = y;
+  P.gate = gate;
+  P.up = up;
+  P.w = w_gate;
+  P.sw = s_gate;
+  P.w2 = w_up;
+  P.sw2 = s_up;
+  return forward(P, x, x_scales, M, N, K, x_dtype, y_dtype, workspace, workspace_bytes,
+                 (hipStream_t)stream);
+}
+
+int mi_int8_matmul_backward(void* dx, const void* dy, const int8_t* w, const float* w_scales,
+                            int64_t M, int64_t N, int64_t K, int dtype, void* workspace,
+                            int64_t workspace_bytes, void* stream) {
+  mi::Int8GradParams G{};
+  mi::Int8BwdParams B{};
+  G.dy = dy;
+  G.sw = w_scales;
+  B.dx = dx;
+  B.w[0] = w;
+  return backward(G, B, M, N, K, dtype, 1, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+int mi_int8_gate_up_swiglu_backward(void* dx, void* dgate, void* dup, const void* dy,
+                                    const void* gate, const void* up, const int8_t* w_gate,
+                                    const float* s_gate, const int8_t* w_up, const float* s_up,
+                                    int64_t M, int64_t N, int64_t K, int dtype, void* workspace,
+                                    int64_t workspace_bytes, void* stream) {
+  mi::Int8GradParams G{};
+  mi::Int8BwdParams B{};
+  G.dy = dy;
+  G.gate = gate;
+  G.up = up;
+  G.sw = s_gate;
+  G.sw2 = s_up;
+  G.dgate = dgate;
+  G.dup = dup;
+  B.dx = dx;
+  B.w[0] = w_gate;
+  B.w[1] = w_up;
+  return backward(G, B, M, N, K, dtype, 2, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,161 @@
+// Int8 products of any size and alignment: 64 x 64 output tiles, operands staged through LDS byte
+// by byte where a 16-byte load could leave the row. The kernels of int8_gemv.hip, int8_gemm.hip and
+// int8_bwd.hip take the aligned layouts; what is left here are rows of K bytes that are no multiple
+// of 16, as no model's are.
+#include "int8.h"
+
+namespace mi {
+namespace {
+
+using namespace i8;
+
+constexpr int kT = 64;        // rows of either operand
+constexpr int kLd = 64 + 16;  // bytes of a staged row: 16-byte aligned, banks spread
+
+// 16 codes k .. k+15 of a row, zeros from K on
+MI_DEV u32x4_t codes16(const int8_t* row, int k, int K, bool aligned) {
+  if (k + 16 <= K && aligned) return *reinterpret_cast<const u32x4_t*>(row + k);
+  u32x4_t v = {0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+    if (k + j < K) v[j / 4] |= (uint32_t)(uint8_t)row[k + j] << (8 * (j % 4));
+  return v;
+}
+
+// y (or the gate and up products): block of 4 waves, wave w rows 16w .. 16w+15 of the weights
+// against all 64 rows of x.
+template <int T, bool DUAL>
+__global__ void __launch_bounds__(256) int8_any_kernel(Int8Params P) {
+  __shared__ __attribute__((aligned(16))) unsigned char xs[kT * kLd];
+  __shared__ __attribute__((aligned(16))) unsigned char ws[(DUAL ? 2 : 1) * kT * kLd];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int fr = lane & 15, q = lane >> 4;
+  const int ntiles = (P.N + kT - 1) / kT;
+  const int64_t m0 = (int64_t)(blockIdx.x / ntiles) * kT;
+  const int n0 = (int)(blockIdx.x % ntiles) * kT;
+  const bool xa = ((uintptr_t)P.x | (uintptr_t)P.ldx) % 16 == 0;
+  const bool wa = ((uintptr_t)P.w | (uintptr_t)(DUAL ? P.w2 : P.w) | (uintptr_t)P.K) % 16 == 0;
+  const int r = tid >> 2, c = 16 * (tid & 3);  // the row and bytes this thread stages
+  const int64_t xm = min(m0 + r, (int64_t)P.M - 1);
+  const int64_t wn = min(n0 + r, P.N - 1);
+  i32x4_t acc[DUAL ? 2 : 1][4];
+#pragma unroll
+  for (int b = 0; b < (DUAL ? 2 : 1); ++b)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[b][i] = i32x4_t{0, 0, 0, 0};
+  for (int k = 0; k < P.K; k += 64) {
+    *reinterpret_cast<u32x4_t*>(xs + r * kLd + c) = codes16(P.x + xm * P.ldx, k + c, P.K, xa);
+    *reinterpret_cast<u32x4_t*>(ws + r * kLd + c) = codes16(P.w + wn * P.K, k + c, P.K, wa);
+    if constexpr (DUAL)
+      *reinterpret_cast<u32x4_t*>(ws + (kT + r) * kLd + c) = codes16(P.w2 + wn * P.K, k + c, P.K, wa);
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < (DUAL ? 2 : 1); ++b) {
+      const u32x4_t w = *reinterpret_cast<const u32x4_t*>(ws + (b * kT + 16 * wave + fr) * kLd + 16 * q);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        acc[b][i] = mfma_i8(w, *reinterpret_cast<const u32x4_t*>(xs + (16 * i + fr) * kLd + 16 * q), acc[b][i]);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t m = m0 + 16 * i + fr;
+    if (m >= P.M) continue;
+    const float sx = P.sx[m];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int n = n0 + 16 * wave + 4 * q + j;
+      if (n >= P.N) continue;
+      finish<T, DUAL>(P, m, n, acc[0][i][j], DUAL ? acc[DUAL ? 1 : 0][i][j] : 0, sx, P.sw[n],
+                      DUAL ? P.sw2[n] : 0.f, !DUAL && P.bias ? load_f<T>(P.bias, n) : 0.f);
+    }
+  }
+}
+
+// dx: 64 rows x 64 codes of the weight rows' K; 32 values of n a step. The weights' tile is
+// turned in LDS (row k, values n) as exact bf16.
+constexpr int kLdB = 40;  // bf16 values of a staged row
+
+template <int T>
+__global__ void __launch_bounds__(256) int8_bwd_any_kernel(Int8BwdParams P) {
+  __shared__ __attribute__((aligned(16))) uint16_t as[kT * kLdB];
+  __shared__ __attribute__((aligned(16))) uint16_t bs[kT * kLdB];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int fr = lane & 15, q = lane >> 4;
+  const int ktiles = (P.K + kT - 1) / kT;
+  const int64_t m0 = (int64_t)(blockIdx.x / ktiles) * kT;
+  const int k0 = (int)(blockIdx.x % ktiles) * kT;
+  const int ar = tid >> 2, ac = 8 * (tid & 3);   // row of a, 8 values of n
+  const int wr = tid >> 3, wc = 8 * (tid & 7);   // value of n, 8 codes of k
+  const int64_t am = min(m0 + ar, (int64_t)P.M - 1);
+  f32x4_t acc[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int seg = 0; seg < P.banks * P.terms; ++seg) {
+    const uint16_t* a = P.a + (int64_t)seg * P.M * P.np;
+    const int8_t* w = P.w[seg / P.terms];
+    for (int n = 0; n < P.N; n += 32) {  // a is zero up to np, a multiple of 32
+      *reinterpret_cast<u32x4_t*>(as + ar * kLdB + ac) =
+          *reinterpret_cast<const u32x4_t*>(a + am * P.np + n + ac);
+      const bool on = n + wr < P.N;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int k = k0 + wc + j;
+        const float f = on && k < P.K ? (float)w[(int64_t)(n + wr) * P.K + k] : 0.f;
+        bs[(wc + j) * kLdB + wr] = (uint16_t)(__float_as_uint(f) >> 16);
+      }
+      __syncthreads();
+      const u32x4_t b = *reinterpret_cast<const u32x4_t*>(bs + (16 * wave + fr) * kLdB + 8 * q);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        acc[i] = mfma16x16x32(
+            as_bf16x8(b), as_bf16x8(*reinterpret_cast<const u32x4_t*>(as + (16 * i + fr) * kLdB + 8 * q)),
+            acc[i]);
+      __syncthreads();
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t m = m0 + 16 * i + fr;
+    if (m >= P.M) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int k = k0 + 16 * wave + 4 * q + j;
+      if (k < P.K) store_f<T>(P.dx, m * P.K + k, acc[i][j]);
+    }
+  }
+}
+
+template <int T>
+hipError_t launch_any(const Int8Params& P, hipStream_t s) {
+  const dim3 grid((unsigned)((((int64_t)P.M + kT - 1) / kT) * ((P.N + kT - 1) / kT)));
+  if (P.w2)
+    hipLaunchKernelGGL((int8_any_kernel<T, true>), grid, dim3(256), 0, s, P);
+  else
+    hipLaunchKernelGGL((int8_any_kernel<T, false>), grid, dim3(256), 0, s, P);
+  return hipGetLastError();
+}
+
+template <int T>
+hipError_t launch_bwd(const Int8BwdParams& P, hipStream_t s) {
+  const dim3 grid((unsigned)((((int64_t)P.M + kT - 1) / kT) * ((P.K + kT - 1) / kT)));
+  hipLaunchKernelGGL((int8_bwd_any_kernel<T>), grid, dim3(256), 0, s, P);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_int8_any(const Int8Params& P, hipStream_t s) {
+  return P.type == kBF16 ? launch_any<kBF16>(P, s)
+         : P.type == kF16 ? launch_any<kF16>(P, s)
+                          : launch_any<kF32>(P, s);
+}
+
+hipError_t launch_int8_bwd_any(const Int8BwdParams& P, hipStream_t s) {
+  return P.type == kBF16 ? launch_bwd<kBF16>(P, s)
+         : P.type == kF16 ? launch_bwd<kF16>(P, s)
+                          : launch_bwd<kF32>(P, s);
+}
+
+}  // namespace mi

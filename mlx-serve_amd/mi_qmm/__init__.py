@@ -12,5 +12,7 @@ from .ops import (quantized_matmul, gather_qmm, dequantize, quantize, fill_randn
                   gather_qmm_gate_up_swiglu,
                   gather_qmv_gate_up_swiglu, gather_qmv_down_reduce, workspace_reserve,
                   workspace_release, library_gemm_calls,
-                  moe_route_gate_up_swiglu, moe_route_grouped)
+                  moe_route_gate_up_swiglu, moe_route_grouped,
+                  int8_quantize, int8_matmul, int8_gate_up_swiglu, int8_matmul_backward,
+                  int8_gate_up_swiglu_backward)
 from .ckpt import Checkpoint, parse_quant_config  # noqa: F401

@@ -5,8 +5,8 @@ import os
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libmi_qmm.so")
 
-MI_OK, MI_ERR_UNSUPPORTED, MI_ERR_INVALID, MI_ERR_HIP = 0, 1, 2, 3
-DT_UINT8, DT_UINT32, DT_FLOAT16, DT_FLOAT32, DT_BFLOAT16 = 1, 3, 9, 10, 12
+MI_OK, MI_ERR_UNSUPPORTED, MI_ERR_INVALID, MI_ERR_HIP, MI_ERR_WORKSPACE = 0, 1, 2, 3, 4
+DT_UINT8, DT_UINT32, DT_INT8, DT_FLOAT16, DT_FLOAT32, DT_BFLOAT16 = 1, 3, 5, 9, 10, 12
 
 
 class MiError(RuntimeError):
@@ -68,6 +68,15 @@ def lib():
     L.mi_moe_route_grouped.argtypes = [P, P, P, P, i64, i64, i32, i32, i32, b, ctypes.c_float, P]
     L.mi_moe_route_gate_up_swiglu.argtypes = [P, P, P, P, P, P, P, P, P, P, P, i64, i64, i32,
                                               i64, i64, OptInt, OptInt, s, i32, P]
+    L.mi_int8_quantize.argtypes = [P, P, P, i64, i64, i32, P]
+    L.mi_int8_forward_workspace.argtypes = [i64, i64, i64, i32, i32]
+    L.mi_int8_forward_workspace.restype = i64
+    L.mi_int8_backward_workspace.argtypes = [i64, i64, i64, i32, i32]
+    L.mi_int8_backward_workspace.restype = i64
+    L.mi_int8_matmul.argtypes = [P] * 6 + [i64, i64, i64, i32, i32, P, i64, P]
+    L.mi_int8_gate_up_swiglu.argtypes = [P] * 9 + [i64, i64, i64, i32, i32, P, i64, P]
+    L.mi_int8_matmul_backward.argtypes = [P] * 4 + [i64, i64, i64, i32, P, i64, P]
+    L.mi_int8_gate_up_swiglu_backward.argtypes = [P] * 10 + [i64, i64, i64, i32, P, i64, P]
     L.mi_workspace_reserve.argtypes = [i64, P]
     L.mi_workspace_release.argtypes = [P]
     L.mi_library_gemm_calls.argtypes = []

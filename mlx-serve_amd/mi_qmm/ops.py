@@ -10,7 +10,8 @@ import math
 
 import torch
 
-from ._lib import (DT_BFLOAT16, DT_FLOAT32, DT_UINT8, MI_ERR_INVALID, MiError, check, lib, opt)
+from ._lib import (DT_BFLOAT16, DT_FLOAT16, DT_FLOAT32, DT_INT8, DT_UINT8, MI_ERR_INVALID, MiError,
+                   check, lib, opt)
 
 _DT = {torch.bfloat16: DT_BFLOAT16, torch.float32: DT_FLOAT32, torch.uint8: DT_UINT8}
 # bias-less microscaling modes: (group_size, bits) each one defines
@@ -398,6 +399,148 @@ def gather_qmv_down_reduce(act, wd, sd, bd, inds, scores, group_size=None, bits=
                                           _ptr(inds), _ptr(scores), T, k, N, K, E, opt(gs),
                                           opt(nb), mode.encode() if mode else None, _stream(act)))
     return y
+
+
+# ------------------------------------------- int8 weights and activations --
+_I8 = {torch.bfloat16: DT_BFLOAT16, torch.float16: DT_FLOAT16, torch.float32: DT_FLOAT32}
+
+
+def _i8_type(dtype, what):
+    if dtype not in _I8:
+        raise MiError(MI_ERR_INVALID, f"{what} dtype {dtype} not supported (bfloat16, float16, float32)")
+    return _I8[dtype]
+
+
+def _i8_linear(N, K, dev, *banks):
+    """Every bank is int8 [N, K] with fp32 scales [N], on the device of the activations."""
+    for w, s in banks:
+        _contig(w, s)
+        _require(w.dtype == torch.int8 and w.dim() == 2, "weights must be int8 [N, K]")
+        _require(w.shape[0] == N and w.shape[1] == K,
+                 f"weights {tuple(w.shape)} do not match [{N}, {K}]")
+        _require(s.dtype == torch.float32 and s.numel() == N, "channel scales must be float32 [N]")
+        _require(w.device == dev and s.device == dev, "tensors on different devices")
+
+
+def _i8_call(fn, dev, need, *args):
+    """One library call on dev's current stream, with a workspace from torch's allocator: calls on
+    other streams and graphs captured from them have others."""
+    if dev.index is not None and dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _i8_call(fn, dev, need, *args)
+    need = max(need, 0)  # sizes out of range: the call refuses them
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    check(fn(*args, _ptr(ws), need, ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)))
+
+
+def int8_quantize(x):
+    """Rows of x [..., K] (bfloat16, float16 or float32) -> (int8 codes [..., K], float32 scales
+    [...]): scale = max |x| / 127, code = the nearest integer to x / scale, ties to even.
+    For the tokens of an activation and for the output channels of a weight [N, K]."""
+    _contig(x)
+    _require(x.dim() >= 1 and x.shape[-1] > 0, "x must be [..., K] with K > 0")
+    code = _i8_type(x.dtype, "x")
+    K = x.shape[-1]
+    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    s = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    L = lib()
+    _i8_call(lambda q, s, x, rows, K, code, ws, need, stream:
+             L.mi_int8_quantize(q, s, x, rows, K, code, stream),
+             x.device, 0, _ptr(q), _ptr(s), _ptr(x), x.numel() // K, K, code)
+    return q, s
+
+
+def _i8_activations(x, x_scales, dtype, K):
+    """(x's code, y's dtype) of a forward call."""
+    _contig(x, x_scales)
+    _require(x.dim() >= 1 and x.shape[-1] == K, f"x {tuple(x.shape)} must end in K={K}")
+    if x.dtype == torch.int8:
+        _require(x_scales is not None, "int8 x needs x_scales")
+        _require(x_scales.dtype == torch.float32 and x_scales.numel() * K == x.numel(),
+                 "x_scales must be float32, one a row of x")
+        _require(x_scales.device == x.device, "tensors on different devices")
+        return DT_INT8, torch.bfloat16 if dtype is None else dtype
+    _require(x_scales is None, "x_scales belong to int8 x")
+    return _i8_type(x.dtype, "x"), x.dtype if dtype is None else dtype
+
+
+def int8_matmul(x, w, w_scales, x_scales=None, bias=None, dtype=None):
+    """y[..., n] = sum_k x[..., k] w[n, k] on the int8 matrix cores. w int8 [N, K] with w_scales
+    [N] (int8_quantize of a weight); x floats, quantized by row within the call, or int8 codes with
+    x_scales. y has `dtype` (default: x's, bfloat16 for codes); bias [N] in it, or None."""
+    _require(w.dim() == 2, "weights must be int8 [N, K]")
+    N, K = w.shape
+    xt, dtype = _i8_activations(x, x_scales, dtype, K)
+    _i8_linear(N, K, x.device, (w, w_scales))
+    yt = _i8_type(dtype, "y")
+    if bias is not None:
+        _contig(bias)
+        _require(bias.dtype == dtype and bias.numel() == N and bias.device == x.device,
+                 "bias must be [N] in y's dtype, on x's device")
+    M = x.numel() // K if K else 0
+    y = torch.empty(x.shape[:-1] + (N,), dtype=dtype, device=x.device)
+    L = lib()
+    _i8_call(L.mi_int8_matmul, x.device, L.mi_int8_forward_workspace(M, N, K, 1, xt), _ptr(y),
+             _ptr(x), _ptr(x_scales), _ptr(w), _ptr(w_scales), _ptr(bias), M, N, K, xt, yt)
+    return y
+
+
+def int8_gate_up_swiglu(x, wg, sg, wu, su, x_scales=None, dtype=None, save=False):
+    """silu(x @ wg.T) * (x @ wu.T) in one launch, operands as int8_matmul. save=True returns
+    (y, gate, up), the two projections for int8_gate_up_swiglu_backward."""
+    _require(wg.dim() == 2, "weights must be int8 [N, K]")
+    N, K = wg.shape
+    xt, dtype = _i8_activations(x, x_scales, dtype, K)
+    _i8_linear(N, K, x.device, (wg, sg), (wu, su))
+    yt = _i8_type(dtype, "y")
+    M = x.numel() // K if K else 0
+    shape = x.shape[:-1] + (N,)
+    y = torch.empty(shape, dtype=dtype, device=x.device)
+    gate = torch.empty(shape, dtype=dtype, device=x.device) if save else None
+    up = torch.empty(shape, dtype=dtype, device=x.device) if save else None
+    L = lib()
+    _i8_call(L.mi_int8_gate_up_swiglu, x.device, L.mi_int8_forward_workspace(M, N, K, 2, xt), _ptr(y),
+             _ptr(gate), _ptr(up), _ptr(x), _ptr(x_scales), _ptr(wg), _ptr(sg), _ptr(wu), _ptr(su),
+             M, N, K, xt, yt)
+    return (y, gate, up) if save else y
+
+
+def int8_matmul_backward(dy, w, w_scales):
+    """The gradient of int8_matmul to x: dx = (dy * w_scales) @ w, dy [..., N] -> [..., K] (weights
+    constant, the rounding of x passed straight through)."""
+    _contig(dy)
+    _require(w.dim() == 2, "weights must be int8 [N, K]")
+    N, K = w.shape
+    _require(dy.dim() >= 1 and dy.shape[-1] == N, f"dy {tuple(dy.shape)} must end in N={N}")
+    _i8_linear(N, K, dy.device, (w, w_scales))
+    code = _i8_type(dy.dtype, "dy")
+    M = dy.numel() // N if N else 0
+    dx = torch.empty(dy.shape[:-1] + (K,), dtype=dy.dtype, device=dy.device)
+    L = lib()
+    _i8_call(L.mi_int8_matmul_backward, dy.device, L.mi_int8_backward_workspace(M, N, K, 1, code),
+             _ptr(dx), _ptr(dy), _ptr(w), _ptr(w_scales), M, N, K, code)
+    return dx
+
+
+def int8_gate_up_swiglu_backward(dy, gate, up, wg, sg, wu, su):
+    """The gradients of int8_gate_up_swiglu(save=True): (dx [..., K], dgate, dup [..., N])."""
+    _contig(dy, gate, up)
+    _require(wg.dim() == 2, "weights must be int8 [N, K]")
+    N, K = wg.shape
+    _require(dy.dim() >= 1 and dy.shape[-1] == N, f"dy {tuple(dy.shape)} must end in N={N}")
+    for t, what in ((gate, "gate"), (up, "up")):
+        _require(t.shape == dy.shape and t.dtype == dy.dtype and t.device == dy.device,
+                 f"{what} must match dy in shape, dtype and device")
+    _i8_linear(N, K, dy.device, (wg, sg), (wu, su))
+    code = _i8_type(dy.dtype, "dy")
+    M = dy.numel() // N if N else 0
+    dx = torch.empty(dy.shape[:-1] + (K,), dtype=dy.dtype, device=dy.device)
+    dgate, dup = torch.empty_like(dy), torch.empty_like(dy)
+    L = lib()
+    _i8_call(L.mi_int8_gate_up_swiglu_backward, dy.device,
+             L.mi_int8_backward_workspace(M, N, K, 2, code), _ptr(dx), _ptr(dgate), _ptr(dup),
+             _ptr(dy), _ptr(gate), _ptr(up), _ptr(wg), _ptr(sg), _ptr(wu), _ptr(su), M, N, K, code)
+    return dx, dgate, dup
 
 
 def library_gemm_calls():

@@ -1,0 +1,98 @@
+"""The int8 operators in 64 bits, from their formulas, and how far a result may be from them.
+
+u = 2^-24 is half a step of fp32; HALF[t] half a step of a type. Bounds are per value and count each
+rounding on the way; `floor` is half of the type's smallest subnormal (fp16 outputs near zero)."""
+import torch
+
+U = 2.0 ** -24
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+FLOOR = {torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -150}
+# bf16 parts of a scaled gradient: what they leave of it
+PARTS = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -16, torch.float32: 2.0 ** -24}
+
+
+def quantize(x):
+    """(codes, scales): the nearest integer to x / s, ties to even. The quotient of two 24-bit
+    numbers is exact enough in 64 bits that a half-integer is met only where it is one."""
+    s = (x.double().abs().amax(-1) / 127).float()
+    q = torch.round(x.double() / s.double().unsqueeze(-1)).clamp(-127, 127)
+    fine = torch.isfinite(s) & (s > 0)
+    return torch.where(fine.unsqueeze(-1), q, torch.zeros_like(q)).to(torch.int8), s
+
+
+def product(q, sx, w, sw):
+    return (q.double() @ w.double().t()) * sx.double()[:, None] * sw.double()[None, :]
+
+
+def check(y, ref, tol, what=""):
+    """|y - ref| <= tol everywhere, not-a-numbers and infinities in the same places."""
+    y, ref = y.double(), ref.double()
+    fine = torch.isfinite(ref)
+    assert torch.equal(torch.isnan(y), torch.isnan(ref)), f"{what}: NaN elsewhere"
+    assert torch.equal(torch.isfinite(y), fine), f"{what}: infinite elsewhere"
+    over = ((y - ref).abs() - tol)[fine]
+    if over.numel():
+        assert over.max().item() <= 0, f"{what}: {over.max().item():.3g} over the bound"
+
+
+def matmul(q, sx, w, sw, bias=None):
+    """(y, tolerance as a function of y's type): the sum is exact; its conversion, two products with
+    scales and the sum with the bias round once each in fp32, then y."""
+    p = product(q, sx, w, sw)
+    y = p if bias is None else p + bias.double()
+    return y, lambda t: 1.01 * (HALF[t] * y.abs() + U * (3 * p.abs() + y.abs())) + FLOOR[t]
+
+
+def gate_up(q, sx, wg, sg, wu, su):
+    """(y, gate, up, tolerance of y, of gate, of up). silu's relative condition number is at most
+    1 + |g|: 3 roundings of g count that much, the exponential is within 2 of its own U (one ulp), and
+    1 + e, the quotient and the products round once each. e^-g overflows below g = -88: 2^-120."""
+    g, u = product(q, sx, wg, sg), product(q, sx, wu, su)
+    y = g * torch.special.expit(g) * u
+    rel = U * (3 * (1 + g.abs()) + 2 * (1 + g.abs()) + 3 + 5)
+
+    def tol(t):
+        return 1.01 * (HALF[t] + rel) * y.abs() + (g * u).abs() * 2.0 ** -120 + FLOOR[t]
+    return (y, g, u, tol) + tuple(
+        (lambda t, v=v: 1.01 * (HALF[t] + 3 * U) * v.abs() + FLOOR[t]) for v in (g, u))
+
+
+def grads(dy, g, u):
+    """(dgate, dup, tolerances before their rounding): s within 5 U of its value (exponential 2, sum,
+    quotient; its exponent's rounding |g| more); 1 - s has that as an absolute error."""
+    dy, g, u = dy.double(), g.double(), u.double()
+    s = torch.special.expit(g)
+    dg, du = dy * u * (s + g * s * (1 - s)), dy * g * s
+    es = U * (5 + g.abs())
+    tg = (dy * u * s).abs() * ((1 + g.abs() * (1 - s)) * (es + 4 * U) + g.abs() * (s * es + 3 * U))
+    tu = du.abs() * (es + 2 * U)
+    tiny = 2.0 ** -120
+    return dg, du, 1.01 * tg + (dy * u).abs() * tiny, 1.01 * tu + (dy * g).abs() * tiny
+
+
+def through(a, ta, w, sw, t):
+    """(sum_n a[m,n] sw[n] w[n,k], its tolerance before the output's rounding): the scaled value rounds
+    once in fp32 and is cut to its bf16 parts; a sum of n terms is off by at most n steps (2 U) of the
+    sum of their magnitudes, parts counted as terms."""
+    b = a * sw.double()[None, :]
+    wd = w.double()
+    n = a.shape[1] * {torch.bfloat16: 1, torch.float16: 2, torch.float32: 3}[t]
+    mag = b.abs() @ wd.abs()
+    err = (ta * sw.double()[None, :].abs()) @ wd.abs()
+    return b @ wd, 1.01 * (mag * (PARTS[t] + U + 2 * U * n) + err)
+
+
+def matmul_backward(dy, w, sw):
+    t = dy.dtype
+    dx, tol = through(dy.double(), torch.zeros_like(dy, dtype=torch.float64), w, sw, t)
+    return dx, 1.01 * HALF[t] * dx.abs() + tol + FLOOR[t]
+
+
+def gate_up_backward(dy, g, u, wg, sg, wu, su):
+    t = dy.dtype
+    dg, du, tg, tu = grads(dy, g, u)
+    a, ta = through(dg, tg, wg, sg, t)
+    b, tb = through(du, tu, wu, su, t)
+    dx = a + b
+    out = lambda v, e: 1.01 * HALF[t] * v.abs() + e + FLOOR[t]
+    return (dx, dg, du), (out(dx, ta + tb), out(dg, tg), out(du, tu))
