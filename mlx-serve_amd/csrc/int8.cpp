@@ -47,12 +47,23 @@ int check_workspace(const void* ws, int64_t given, int64_t need) {
   return MI_OK;
 }
 
-// Forward workspace: codes [M, ldx], then scales, of activations that come as floats.
+// Forward workspace: codes [M, ldx] and scales of activations that come as floats, then the K
+// ranges' sums of a split product. Sizes alone decide what is asked for; a call on pointers
+// that another kernel has to take leaves the sums' part unused.
 int64_t codes_bytes(int64_t M, int64_t K) { return up(M * up(K, 16), 256); }
-int64_t forward_need(int64_t M, int64_t K, int x_dtype) {
-  if (x_dtype == MI_DTYPE_INT8 || M == 0) return 0;
-  return codes_bytes(M, K) + M * 4;
+int64_t quant_bytes(int64_t M, int64_t K, int x_dtype) {
+  return x_dtype == MI_DTYPE_INT8 ? 0 : codes_bytes(M, K) + up(M * 4, 256);
 }
+int64_t forward_need(mi::Int8Params& P, int64_t M, int64_t N, int64_t K, int x_dtype) {
+  if (M == 0 || N == 0 || K == 0) return 0;
+  P.M = (int)M;
+  P.N = (int)N;
+  P.K = (int)K;
+  P.ks = 1;
+  if (K % 16 == 0) mi::int8_gemm_plan(P);
+  return quant_bytes(M, K, x_dtype) + (P.ks > 1 ? (int64_t)P.ks * P.banks * M * N * 4 : 0);
+}
+bool aligned(const void* p, int a) { return (uintptr_t)p % a == 0; }
 
 int forward(mi::Int8Params& P, const void* x, const float* x_scales, int64_t M, int64_t N,
             int64_t K, int x_dtype, int y_dtype, void* ws, int64_t ws_bytes, hipStream_t s) {
@@ -70,10 +81,11 @@ int forward(mi::Int8Params& P, const void* x, const float* x_scales, int64_t M, 
   if (((M + 63) / 64) * ((N + 63) / 64) > kMaxTiles)
     return report_error(MI_ERR_UNSUPPORTED, "M * N too large for one call");
   if (!P.y || !x || !P.w || !P.sw || (xt < 0 && !x_scales)) return bad("null tensor pointer");
-  if (int rc = check_workspace(ws, ws_bytes, forward_need(M, K, x_dtype))) return rc;
-  P.M = (int)M;
-  P.N = (int)N;
-  P.K = (int)K;
+  P.banks = P.w2 ? 2 : 1;
+  if (int rc = check_workspace(ws, ws_bytes, forward_need(P, M, N, K, x_dtype))) return rc;
+  P.part = (int32_t*)((char*)ws + quant_bytes(M, K, x_dtype));
+  const int a4 = P.type == mi::kF32 ? 16 : 8;
+  P.vec = N % 4 == 0 && aligned(P.y, a4) && aligned(P.gate, a4) && aligned(P.up, a4);
   P.x = (const int8_t*)x;
   P.sx = x_scales;
   P.ldx = K;
@@ -84,7 +96,9 @@ int forward(mi::Int8Params& P, const void* x, const float* x_scales, int64_t M, 
     const hipError_t e = mi::launch_int8_quantize((int8_t*)ws, (float*)P.sx, x, M, K, P.ldx, xt, s);
     if (e != hipSuccess) return hip_status(e, "int8 quantize launch");
   }
-  return hip_status(mi::launch_int8_any(P, s), "int8 matmul launch");
+  return hip_status(mi::int8_gemm_supported(N, K, P.x, P.ldx, P.w, P.w2) ? mi::launch_int8_gemm(P, s)
+                                                                         : mi::launch_int8_any(P, s),
+                    "int8 matmul launch");
 }
 
 // Backward workspace: the bf16 parts of the incoming gradient, [banks * terms][M][np].
@@ -139,8 +153,12 @@ int mi_int8_quantize(int8_t* q, float* scales, const void* x, int64_t rows, int6
 }
 
 int64_t mi_int8_forward_workspace(int64_t M, int64_t N, int64_t K, int banks, int x_dtype) {
-  if (M < 0 || N < 0 || K < 0 || banks < 1 || banks > 2 || M > kMaxDim || K > kMaxDim) return -1;
-  return forward_need(M, K, x_dtype);
+  if (M < 0 || N < 0 || K < 0 || banks < 1 || banks > 2 || M > kMaxDim || N > kMaxDim ||
+      K > mi::kInt8MaxK || ((M + 63) / 64) * ((N + 63) / 64) > kMaxTiles)
+    return -1;
+  mi::Int8Params P{};
+  P.banks = banks;
+  return forward_need(P, M, N, K, x_dtype);
 }
 
 int64_t mi_int8_backward_workspace(int64_t M, int64_t N, int64_t K, int banks, int dtype) {

@@ -29,7 +29,13 @@ struct Int8Params {
   int xf_type;
   int64_t ldx;
   int M, N, K;
-  int type;  // FloatType of y, bias, gate and up
+  int type;   // FloatType of y, bias, gate and up
+  int banks;  // 1, or 2 with w2
+  // int8_gemm.hip: rows of a tile; K ranges over blocks and 128-code steps of one, ks > 1
+  // through int32 sums [ks][banks][M][N] in `part`
+  int bm, ks, sps;
+  int32_t* part;
+  bool vec;  // y, gate, up, part rows of four columns on one store (N and pointers)
 };
 
 // dx[m,k] = sum over banks and n of a[m,n] w[n,k], a split into `terms` bf16 parts:
@@ -62,6 +68,10 @@ struct Int8GradParams {
 
 hipError_t launch_int8_quantize(int8_t* q, float* s, const void* x, int64_t rows, int64_t K,
                                 int64_t ldq, int type, hipStream_t st);
+bool int8_gemm_supported(int64_t N, int64_t K, const void* x, int64_t ldx, const void* w,
+                         const void* w2);
+void int8_gemm_plan(Int8Params& P);  // from M, N, K and banks: bm, ks, sps
+hipError_t launch_int8_gemm(const Int8Params& P, hipStream_t s);
 hipError_t launch_int8_any(const Int8Params& P, hipStream_t s);
 hipError_t launch_int8_grad(const Int8GradParams& P, hipStream_t s);
 hipError_t launch_int8_bwd_any(const Int8BwdParams& P, hipStream_t s);
@@ -96,22 +106,104 @@ MI_DEV i32x4_t mfma_i8(u32x4_t a, u32x4_t b, i32x4_t c) {
 // 1 / (1 + e^-g): e^-g overflows to infinity for g < -88, which gives 0, the limit.
 MI_DEV float sigmoid_f(float g) { return 1.f / (1.f + expf(-g)); }
 
-// The products of one output, to memory. Scales are applied in 32 bits, one rounding at the end.
-template <int T, bool DUAL>
-MI_DEV void finish(const Int8Params& P, int64_t m, int n, int32_t a, int32_t b, float sx,
-                   float sw, float sw2, float bias) {
-  const int64_t i = m * P.N + n;
-  const float g = (float)a * sx * sw;
-  if constexpr (!DUAL) {
-    store_f<T>(P.y, i, g + bias);
+// Four neighbouring values, one rounding each; `vec`: with one store.
+MI_DEV void store4(void* p, int64_t i, int type, bool vec, int cnt, const float (&v)[4]) {
+  if (type == kF32) {
+    float* o = (float*)p + i;
+    if (vec) {
+      *reinterpret_cast<f32x4_t*>(o) = f32x4_t{v[0], v[1], v[2], v[3]};
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < cnt) o[j] = v[j];
+    }
+    return;
+  }
+  uint32_t b[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    b[j] = type == kBF16 ? f32_to_bf16_bits(v[j]) : __builtin_bit_cast(uint16_t, (_Float16)v[j]);
+  uint16_t* o = (uint16_t*)p + i;
+  if (vec) {
+    *reinterpret_cast<u32x2_t*>(o) = u32x2_t{b[0] | b[1] << 16, b[2] | b[3] << 16};
   } else {
-    const float u = (float)b * sx * sw2;
-    store_f<T>(P.y, i, g * sigmoid_f(g) * u);
-    if (P.gate) {
-      store_f<T>(P.gate, i, g);
-      store_f<T>(P.up, i, u);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < cnt) o[j] = (uint16_t)b[j];
+  }
+}
+MI_DEV float load_rt(const void* p, int64_t i, int type) {
+  return type == kBF16 ? load_f<kBF16>(p, i) : type == kF16 ? load_f<kF16>(p, i) : load_f<kF32>(p, i);
+}
+
+// Scales and bias of columns n .. n + 3 (those from N on repeat column n).
+struct Cols {
+  float s[4], s2[4], b[4];
+};
+template <bool DUAL>
+MI_DEV Cols load_cols(const Int8Params& P, int n) {
+  Cols c;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int k = n + j < P.N ? n + j : n;
+    c.s[j] = P.sw[k];
+    c.s2[j] = DUAL ? P.sw2[k] : 0.f;
+    c.b[j] = !DUAL && P.bias ? load_rt(P.bias, k, P.type) : 0.f;
+  }
+  return c;
+}
+
+// The sums of columns n .. n + 3 (those below N) of row m, to memory: scales in 32 bits, one
+// rounding at the end.
+template <bool DUAL>
+MI_DEV void finish4(const Int8Params& P, int64_t m, int n, i32x4_t a, i32x4_t b, float sx, const Cols& c) {
+  const int64_t i = m * P.N + n;
+  const int cnt = P.N - n;
+  float y[4], u[4], g[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    g[j] = (float)a[j] * sx * c.s[j];
+    if constexpr (DUAL) {
+      u[j] = (float)b[j] * sx * c.s2[j];
+      y[j] = g[j] * sigmoid_f(g[j]) * u[j];
+    } else {
+      y[j] = P.bias ? g[j] + c.b[j] : g[j];
     }
   }
+  store4(P.y, i, P.type, P.vec, cnt, y);
+  if constexpr (DUAL) {
+    if (P.gate) {
+      store4(P.gate, i, P.type, P.vec, cnt, g);
+      store4(P.up, i, P.type, P.vec, cnt, u);
+    }
+  }
+}
+
+// int32 sums of a K range: [split][bank][M][N]
+template <bool DUAL>
+MI_DEV void store_part(const Int8Params& P, int split, int64_t m, int n, i32x4_t a, i32x4_t b) {
+#pragma unroll
+  for (int k = 0; k < (DUAL ? 2 : 1); ++k) {
+    int32_t* o = P.part + (((int64_t)split * (DUAL ? 2 : 1) + k) * P.M + m) * P.N + n;
+    const i32x4_t v = k ? b : a;
+    if (P.N % 4 == 0) {
+      *reinterpret_cast<i32x4_t*>(o) = v;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (n + j < P.N) o[j] = v[j];
+    }
+  }
+}
+template <bool DUAL>
+MI_DEV i32x4_t load_part(const Int8Params& P, int split, int bank, int64_t m, int n) {
+  const int32_t* p = P.part + (((int64_t)split * (DUAL ? 2 : 1) + bank) * P.M + m) * P.N + n;
+  if (P.N % 4 == 0) return *reinterpret_cast<const i32x4_t*>(p);
+  i32x4_t v = {0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (n + j < P.N) v[j] = p[j];
+  return v;
 }
 
 }  // namespace i8

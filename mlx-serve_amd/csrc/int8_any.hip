@@ -24,7 +24,7 @@ MI_DEV u32x4_t codes16(const int8_t* row, int k, int K, bool aligned) {
 
 // y (or the gate and up products): block of 4 waves, wave w rows 16w .. 16w+15 of the weights
 // against all 64 rows of x.
-template <int T, bool DUAL>
+template <bool DUAL>
 __global__ void __launch_bounds__(256) int8_any_kernel(Int8Params P) {
   __shared__ __attribute__((aligned(16))) unsigned char xs[kT * kLd];
   __shared__ __attribute__((aligned(16))) unsigned char ws[(DUAL ? 2 : 1) * kT * kLd];
@@ -35,7 +35,7 @@ __global__ void __launch_bounds__(256) int8_any_kernel(Int8Params P) {
   const int n0 = (int)(blockIdx.x % ntiles) * kT;
   const bool xa = ((uintptr_t)P.x | (uintptr_t)P.ldx) % 16 == 0;
   const bool wa = ((uintptr_t)P.w | (uintptr_t)(DUAL ? P.w2 : P.w) | (uintptr_t)P.K) % 16 == 0;
-  const int r = tid >> 2, c = 16 * (tid & 3);  // the row and bytes this thread stages
+  const int r = tid >> 2, rb = 16 * (tid & 3);  // the row and bytes this thread stages
   const int64_t xm = min(m0 + r, (int64_t)P.M - 1);
   const int64_t wn = min(n0 + r, P.N - 1);
   i32x4_t acc[DUAL ? 2 : 1][4];
@@ -44,10 +44,10 @@ __global__ void __launch_bounds__(256) int8_any_kernel(Int8Params P) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[b][i] = i32x4_t{0, 0, 0, 0};
   for (int k = 0; k < P.K; k += 64) {
-    *reinterpret_cast<u32x4_t*>(xs + r * kLd + c) = codes16(P.x + xm * P.ldx, k + c, P.K, xa);
-    *reinterpret_cast<u32x4_t*>(ws + r * kLd + c) = codes16(P.w + wn * P.K, k + c, P.K, wa);
+    *reinterpret_cast<u32x4_t*>(xs + r * kLd + rb) = codes16(P.x + xm * P.ldx, k + rb, P.K, xa);
+    *reinterpret_cast<u32x4_t*>(ws + r * kLd + rb) = codes16(P.w + wn * P.K, k + rb, P.K, wa);
     if constexpr (DUAL)
-      *reinterpret_cast<u32x4_t*>(ws + (kT + r) * kLd + c) = codes16(P.w2 + wn * P.K, k + c, P.K, wa);
+      *reinterpret_cast<u32x4_t*>(ws + (kT + r) * kLd + rb) = codes16(P.w2 + wn * P.K, k + rb, P.K, wa);
     __syncthreads();
 #pragma unroll
     for (int b = 0; b < (DUAL ? 2 : 1); ++b) {
@@ -58,18 +58,13 @@ __global__ void __launch_bounds__(256) int8_any_kernel(Int8Params P) {
     }
     __syncthreads();
   }
+  const int n = n0 + 16 * wave + 4 * q;
+  if (n >= P.N) return;
+  const Cols c = load_cols<DUAL>(P, n);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int64_t m = m0 + 16 * i + fr;
-    if (m >= P.M) continue;
-    const float sx = P.sx[m];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int n = n0 + 16 * wave + 4 * q + j;
-      if (n >= P.N) continue;
-      finish<T, DUAL>(P, m, n, acc[0][i][j], DUAL ? acc[DUAL ? 1 : 0][i][j] : 0, sx, P.sw[n],
-                      DUAL ? P.sw2[n] : 0.f, !DUAL && P.bias ? load_f<T>(P.bias, n) : 0.f);
-    }
+    if (m < P.M) finish4<DUAL>(P, m, n, acc[0][i], acc[DUAL ? 1 : 0][i], P.sx[m], c);
   }
 }
 
@@ -128,16 +123,6 @@ __global__ void __launch_bounds__(256) int8_bwd_any_kernel(Int8BwdParams P) {
 }
 
 template <int T>
-hipError_t launch_any(const Int8Params& P, hipStream_t s) {
-  const dim3 grid((unsigned)((((int64_t)P.M + kT - 1) / kT) * ((P.N + kT - 1) / kT)));
-  if (P.w2)
-    hipLaunchKernelGGL((int8_any_kernel<T, true>), grid, dim3(256), 0, s, P);
-  else
-    hipLaunchKernelGGL((int8_any_kernel<T, false>), grid, dim3(256), 0, s, P);
-  return hipGetLastError();
-}
-
-template <int T>
 hipError_t launch_bwd(const Int8BwdParams& P, hipStream_t s) {
   const dim3 grid((unsigned)((((int64_t)P.M + kT - 1) / kT) * ((P.K + kT - 1) / kT)));
   hipLaunchKernelGGL((int8_bwd_any_kernel<T>), grid, dim3(256), 0, s, P);
@@ -147,9 +132,12 @@ hipError_t launch_bwd(const Int8BwdParams& P, hipStream_t s) {
 }  // namespace
 
 hipError_t launch_int8_any(const Int8Params& P, hipStream_t s) {
-  return P.type == kBF16 ? launch_any<kBF16>(P, s)
-         : P.type == kF16 ? launch_any<kF16>(P, s)
-                          : launch_any<kF32>(P, s);
+  const dim3 grid((unsigned)((((int64_t)P.M + kT - 1) / kT) * ((P.N + kT - 1) / kT)));
+  if (P.w2)
+    hipLaunchKernelGGL((int8_any_kernel<true>), grid, dim3(256), 0, s, P);
+  else
+    hipLaunchKernelGGL((int8_any_kernel<false>), grid, dim3(256), 0, s, P);
+  return hipGetLastError();
 }
 
 hipError_t launch_int8_bwd_any(const Int8BwdParams& P, hipStream_t s) {

@@ -1,0 +1,311 @@
+// Int8 products of more than a few rows, on the matrix cores:
+//   acc[m,n] = sum_k x[m,k] w[n,k] (int32, exact), scaled as it is written (int8.h), or for two
+//   banks of weights y = silu(gate) * up of the two sums, which meet in the same lane.
+//
+// Block: 8 waves as 2 (rows of x) x 4 (rows of w), BM x BN outputs, v_mfma_i32_16x16x64_i8 with
+// D[n][m] = w[n][k] x[m][k]. With two banks the 16-row tiles of w alternate gate, up. A step is
+// 128 codes of K: a row of either operand is one cache line, moved by LDS DMA (16 bytes a lane,
+// slots XOR-swizzled by row) into a ring of R stages, and read as fragments half a step ahead
+// of the products that take them. Each half step's products (MT x NT of them a wave) carry the
+// LDS reads of the next half and the DMA; one barrier a step, in its middle: every wave is past
+// its last read of stage t (it sits in registers), so the DMA of stage t + R may go out into it,
+// and stage t + 1 has landed. Vector memory operations return in order, so "landed" is an
+// exact vmcnt.
+//
+// What bounds it: the DMA. Without it the same loop runs 8192 x 4096 x 14336 in 321 us, alone it
+// takes 389 us, together 414: the 64 KB of a step come late when their lines come from HBM or
+// the memory-side cache. So each block asks the L2 for its lines two steps before it moves them
+// (one dword a line, into a corner of LDS that nothing reads), and the blocks of a panel that
+// share a tile of x or w (prefill_tiles.h) each ask for a part of it: alone 292 us, together 398
+// (2.4 POPS; 420 in a row at the clock that the card's power allows then).
+// Against 64-byte steps in a ring of five stages (444 us) and weights straight into registers
+// (455 us).
+//
+// K: any multiple of 16. In the last step the slots from K on load out of bounds, as zeros.
+#include <algorithm>
+
+#include "int8.h"
+#include "prefill_tiles.h"
+#include "qmv_common.h"
+
+namespace mi {
+namespace {
+
+using namespace i8;
+using qmv_detail::vmcnt_imm;
+
+constexpr int kBufFlags = 0x00020000;   // raw dword access
+constexpr uint32_t kOOB = 0x7FFFFFF0u;  // past any resource: the load returns 0
+constexpr int kBK = 128;
+
+// XOR swizzle of the 16-byte slots of a 128-byte row. A ds_read_b128 pass serves lanes 0-3, 12-15,
+// 20-23 and 24-27 of a half together: rows 0-3 and 12-15 of quarter q, 4-11 of quarter q + 1.
+// With slots 2q + e these keep apart.
+MI_DEV int xswz(int r) { return (r & 2) | ((r >> 2) & 1) | ((r >> 1) & 4); }
+
+MI_DEV void dma16(__amdgpu_buffer_rsrc_t rs, unsigned char* lds, uint32_t voff, int soff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)lds, 16,
+                                           voff, soff, 0, 0);
+}
+MI_DEV void dma4(__amdgpu_buffer_rsrc_t rs, unsigned char* lds, uint32_t voff, int soff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)lds, 4,
+                                           voff, soff, 0, 0);
+}
+MI_DEV __amdgpu_buffer_rsrc_t rsrc(const void* p, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, bytes, kBufFlags);
+}
+
+// s_waitcnt vmcnt(n); n is a constant after inlining
+MI_DEV void wait_vm(int n) {
+  switch (n) {
+#define C(n) case n: __builtin_amdgcn_s_waitcnt(vmcnt_imm(n)); break;
+    C(1) C(2) C(3) C(4) C(5) C(6) C(7) C(8) C(9) C(10) C(11) C(12) C(13) C(14) C(15) C(16) C(17)
+    C(18) C(19) C(20) C(21) C(22) C(23) C(24) C(25) C(26) C(27) C(28)
+    default: __builtin_amdgcn_s_waitcnt(vmcnt_imm(0)); break;
+#undef C
+  }
+}
+
+template <int BM, int BN, int R>
+constexpr int lds_bytes() { return R * (BM + BN) * kBK + 2048; }
+
+template <bool DUAL, int BM, int BN, int R, bool SPLIT>
+__global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
+int8_gemm_kernel(Int8Params P) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  constexpr int MT = BM / 32, NT = BN / 64;    // 16-row tiles of a wave
+  constexpr int XI = BM / 64, WI = BN / 64;    // DMA instructions (8 rows) of a wave a step
+  constexpr int kStage = (BM + BN) * kBK, kW = BM * kBK;
+  constexpr int kON = DUAL ? BN / 2 : BN;      // columns of y
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave >> 2, wn = wave & 3;
+  const int fr = lane & 15, q = lane >> 4;
+  const int M = P.M, N = P.N, K = P.K, ldx = (int)P.ldx;
+  const int mtiles = (M + BM - 1) / BM;
+  const TileOf at = tile_of_block(mtiles, (N + kON - 1) / kON);
+  const int m0 = at.mt * BM, n0 = at.nt * kON, s0 = at.split * P.sps;
+  const int ns = min(P.sps, (K + kBK - 1) / kBK - s0);
+  const int mrows = min(BM, M - m0), nrows = min(kON, N - n0);
+  const int xbytes = mrows * ldx, wbytes = nrows * K;
+  const int8_t* xb = P.x + (size_t)m0 * ldx;
+  const int8_t* wb = P.w + (size_t)n0 * K;
+  const int8_t* wb2 = DUAL ? P.w2 + (size_t)n0 * K : wb;
+
+  uint32_t xo[XI], wo[WI];
+  int xc[XI], wc[WI];
+#pragma unroll
+  for (int i = 0; i < XI; ++i) {
+    const int r = 8 * (wave * XI + i) + (lane >> 3);
+    xc[i] = 16 * ((lane & 7) ^ xswz(r));
+    xo[i] = (uint32_t)(min(r, mrows - 1) * ldx + xc[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < WI; ++i) {
+    const int r = 8 * (wave * WI + i) + (lane >> 3);
+    const int row = DUAL ? 16 * (r >> 5) + (r & 15) : r;  // tiles alternate gate, up
+    wc[i] = 16 * ((lane & 7) ^ xswz(r));
+    wo[i] = (uint32_t)min(row, nrows - 1) * (uint32_t)K + wc[i];
+  }
+  // stages past the range load through a resource of zero records (zeros, no traffic)
+  auto issue = [&](int st, int slot) __attribute__((always_inline)) {
+    const bool on = st < ns;
+    const int k = (s0 + st) * kBK;
+    unsigned char* b = smem + slot * kStage;
+#pragma unroll
+    for (int i = 0; i < XI; ++i)
+      dma16(rsrc(xb, on ? xbytes : 0), b + (wave * XI + i) * 1024, xc[i] < K - k ? xo[i] : kOOB, k);
+#pragma unroll
+    for (int i = 0; i < WI; ++i)
+      dma16(rsrc(DUAL && ((wave * WI + i) >> 1 & 1) ? wb2 : wb, on ? wbytes : 0),
+            b + kW + (wave * WI + i) * 1024, wc[i] < K - k ? wo[i] : kOOB, k);
+  };
+  // L2 prefetch: waves 0-3 the rows of x, 4-7 those of w (4, 5 gate and 6, 7 up), 64 a wave. The h
+  // blocks of a panel that read this w tile split its rows, four of those that read x its.
+  const int h = min(4, mtiles - at.mt / 4 * 4);
+  const bool pw = wave >= 4;
+  const int8_t* pb = !pw ? xb : DUAL && (wave & 2) ? wb2 : wb;
+  const int pr = (wave & (DUAL && pw ? 1 : 3)) * 64 + lane, pn = pw ? min(kON, nrows) : min(BM, mrows);
+  const bool mine = pr < pn && (pw ? at.mt % h == (wave & 3) % h : (at.nt & 3) == (wave & 3));
+  const uint32_t po = mine ? (uint32_t)pr * (uint32_t)(pw ? K : ldx) : kOOB;
+  auto prefetch = [&](int st) __attribute__((always_inline)) {
+    dma4(rsrc(pb, st < ns ? (pw ? wbytes : xbytes) : 0), smem + R * kStage + wave * 256, po, (s0 + st) * kBK);
+  };
+
+  i32x4_t acc[NT][MT];
+#pragma unroll
+  for (int a = 0; a < NT; ++a)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[a][i] = i32x4_t{0, 0, 0, 0};
+  u32x4_t X[2][MT], A[2][NT];
+  // half e of a step: slot 2q + e of a row (both operands take the same 64 codes)
+  const int fo0 = fr * kBK + (((2 * q) ^ xswz(fr)) << 4), fo1 = fr * kBK + (((2 * q + 1) ^ xswz(fr)) << 4);
+  const int xr = 16 * wm * MT * kBK, wr = kW + 16 * wn * NT * kBK;
+  auto frags = [&](int slot, int e) __attribute__((always_inline)) {
+    const unsigned char* b = smem + slot * kStage + (e ? fo1 : fo0);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) X[e][i] = *reinterpret_cast<const u32x4_t*>(b + xr + 16 * i * kBK);
+#pragma unroll
+    for (int a = 0; a < NT; ++a) A[e][a] = *reinterpret_cast<const u32x4_t*>(b + wr + 16 * a * kBK);
+  };
+  auto products = [&](int e) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int a = 0; a < NT; ++a) acc[a][i] = mfma_i8(A[e][a], X[e][i], acc[a][i]);
+  };
+
+#pragma unroll
+  for (int s = 0; s < R; ++s) {
+    issue(s, s);
+    prefetch(s + R);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  wait_vm(1 + (R - 1) * (XI + WI + 1));
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  frags(0, 0);
+  int slot = 0;
+#pragma unroll 1
+  for (int t = 0; t < ns; ++t) {
+    const int next = R == 2 ? slot ^ 1 : slot + 1 == R ? 0 : slot + 1;
+    frags(slot, 1);
+    products(0);
+#pragma unroll
+    for (int r = 0; r < MT + NT; ++r) {  // a read, one or two products
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      if (MT * NT >= 2 * (MT + NT)) __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): this wave's reads of stage t
+    wait_vm(1 + (R - 2) * (XI + WI + 1));
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    frags(next, 0);
+    issue(t + R, slot);
+    prefetch(t + 2 * R);
+    products(1);
+#pragma unroll
+    for (int r = 0; r < MT + NT; ++r) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      if (MT * NT >= 2 * (MT + NT)) __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      if (r % 3 != 2) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    slot = next;
+  }
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // no DMA may outlive the block
+
+  // acc[a][i] register j is [n = 16 (wn NT + a) + 4q + j][m = 16 (wm MT + i) + fr]
+  const int mw = m0 + 16 * wm * MT + fr;
+  float sx[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) sx[i] = P.sx[min(mw + 16 * i, M - 1)];
+#pragma unroll
+  for (int a = 0; a < NT; a += DUAL ? 2 : 1) {
+    const int n = n0 + 16 * (DUAL ? (wn * NT + a) / 2 : wn * NT + a) + 4 * q;
+    if (n >= N) continue;
+    const Cols c = load_cols<DUAL>(P, n);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int m = mw + 16 * i;
+      if (m >= M) continue;
+      if constexpr (SPLIT)
+        store_part<DUAL>(P, at.split, m, n, acc[a][i], acc[DUAL ? a + 1 : a][i]);
+      else
+        finish4<DUAL>(P, m, n, acc[a][i], acc[DUAL ? a + 1 : a][i], sx[i], c);
+    }
+  }
+}
+
+// The splits' sums, exact in any order, and the scales.
+template <bool DUAL>
+__global__ void __launch_bounds__(256) int8_reduce_kernel(Int8Params P) {
+  const int64_t n4 = ((int64_t)P.N + 3) / 4, total = n4 * P.M;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t m = i / n4;
+    const int n = (int)(i - m * n4) * 4;
+    i32x4_t a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
+    for (int s = 0; s < P.ks; ++s) {
+      a += load_part<DUAL>(P, s, 0, m, n);
+      if constexpr (DUAL) b += load_part<DUAL>(P, s, 1, m, n);
+    }
+    finish4<DUAL>(P, m, n, a, b, P.sx[m], load_cols<DUAL>(P, n));
+  }
+}
+
+template <bool DUAL, int BM, int BN, int R>
+hipError_t launch_tile(const Int8Params& P, hipStream_t s) {
+  constexpr int lds = lds_bytes<BM, BN, R>();
+  constexpr int kON = DUAL ? BN / 2 : BN;
+  static std::atomic<uint64_t> done{0};  // devices whose functions have the attribute
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  const uint64_t bit = (uint64_t)1 << (dev & 63);
+  if (e == hipSuccess && !(done.load() & bit)) {
+    for (auto k : {int8_gemm_kernel<DUAL, BM, BN, R, false>, int8_gemm_kernel<DUAL, BM, BN, R, true>})
+      if (e == hipSuccess)
+        e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e == hipSuccess) done |= bit;
+  }
+  if (e != hipSuccess) return e;
+  const dim3 grid((unsigned)(((P.M + BM - 1) / BM) * ((P.N + kON - 1) / kON)), (unsigned)P.ks);
+  if (P.ks > 1)
+    hipLaunchKernelGGL((int8_gemm_kernel<DUAL, BM, BN, R, true>), grid, dim3(512), lds, s, P);
+  else
+    hipLaunchKernelGGL((int8_gemm_kernel<DUAL, BM, BN, R, false>), grid, dim3(512), lds, s, P);
+  return hipGetLastError();
+}
+
+template <bool DUAL>
+hipError_t launch_gemm(const Int8Params& P, hipStream_t s) {
+  hipError_t e = P.bm == 256   ? launch_tile<DUAL, 256, 256, 2>(P, s)
+                 : P.bm == 128 ? launch_tile<DUAL, 128, 256, 3>(P, s)
+                               : launch_tile<DUAL, 64, 128, 4>(P, s);
+  if (e != hipSuccess || P.ks == 1) return e;
+  int64_t g = ((int64_t)P.M * ((P.N + 3) / 4) + 255) / 256;
+  if (g > 8192) g = 8192;
+  hipLaunchKernelGGL((int8_reduce_kernel<DUAL>), dim3((unsigned)g), dim3(256), 0, s, P);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+// Rows on 16 bytes and offsets of a tile within 31 bits.
+bool int8_gemm_supported(int64_t N, int64_t K, const void* x, int64_t ldx, const void* w, const void* w2) {
+  return ((uintptr_t)x | (uintptr_t)ldx | (uintptr_t)w | (uintptr_t)w2 | (uintptr_t)K) % 16 == 0;
+}
+
+// Tile and K splits: the fewest estimated microseconds over rounds of 256 blocks (one a CU) x
+// steps, plus a split's int32 partials written and read back and the reduce launch. Depends
+// on the sizes alone (not on pointers), so the workspace can be asked for ahead.
+void int8_gemm_plan(Int8Params& P) {
+  const int steps = (P.K + kBK - 1) / kBK;
+  const int banks = P.banks;
+  struct Tile { int bm, bn; double us; };
+  constexpr Tile kTiles[] = {{256, 256, 1.8}, {128, 256, 1.1}, {64, 128, 0.55}};
+  double best = 1e30;
+  for (const Tile& t : kTiles) {
+    const int on = t.bn / banks;
+    const int64_t tiles = (int64_t)((P.M + t.bm - 1) / t.bm) * ((P.N + on - 1) / on);
+    for (int k = 1; k <= std::max(1, steps / 4) && k <= 64; ++k) {
+      const int sps = (steps + k - 1) / k, ks = (steps + sps - 1) / sps;
+      const double part = ks > 1 ? (double)ks * banks * P.M * P.N * 8 / 5e6 + 4.0 : 0.0;
+      const double cost = (double)((tiles * ks + 255) / 256) * (sps * t.us + 2.0) + part;
+      if (cost < best - 1e-9) {
+        best = cost;
+        P.bm = t.bm;
+        P.ks = ks;
+        P.sps = sps;
+      }
+    }
+  }
+}
+
+hipError_t launch_int8_gemm(const Int8Params& P, hipStream_t s) {
+  return P.w2 ? launch_gemm<true>(P, s) : launch_gemm<false>(P, s);
+}
+
+}  // namespace mi
