@@ -15,7 +15,11 @@ using mi::report_error;
 
 constexpr int64_t kMaxDim = (int64_t)1 << 30;
 constexpr int64_t kMaxTiles = (int64_t)1 << 22;  // blocks of up to 512 threads: below 2^32 threads
-constexpr int64_t kMaxArea = (int64_t)1 << 40;   // values of a gradient
+
+// A backward call's blocks, and offsets within 256 rows of a gradient or 64 of codes below 2^31.
+bool backward_fits(int64_t M, int64_t N, int64_t K) {
+  return ((M + 63) / 64) * ((K + 63) / 64) <= kMaxTiles && N < (int64_t)1 << 21 && K < (int64_t)1 << 24;
+}
 
 int bad(const char* msg) { return report_error(MI_ERR_INVALID, msg); }
 int hip_status(hipError_t e, const char* what) {
@@ -101,10 +105,22 @@ int forward(mi::Int8Params& P, const void* x, const float* x_scales, int64_t M, 
                     "int8 matmul launch");
 }
 
-// Backward workspace: the bf16 parts of the incoming gradient, [banks * terms][M][np].
-int64_t np_of(int64_t N) { return up(N, 64); }
-int64_t backward_need(int64_t M, int64_t N, int banks, int type) {
-  return up(banks * (type + 1) * M * np_of(N) * 2, 256);
+// Backward workspace: the fp16 parts of the scaled gradients, [banks * terms][M][np], the rows'
+// powers of two, then the ranges' sums of a split product. Two parts for fp32, one otherwise.
+int64_t parts_bytes(const mi::Int8BwdParams& B) { return up((int64_t)B.banks * B.terms * B.M * B.np * 2, 256); }
+int64_t rows_bytes(const mi::Int8BwdParams& B) { return up((int64_t)B.M * 4, 256); }
+int64_t backward_need(mi::Int8BwdParams& B, int64_t M, int64_t N, int64_t K, int banks, int type) {
+  if (M == 0 || N == 0 || K == 0) return 0;
+  B.banks = banks;
+  B.terms = type == mi::kF32 ? 2 : 1;
+  B.np = (int)up(N, 64);
+  B.M = (int)M;
+  B.N = (int)N;
+  B.K = (int)K;
+  B.type = type;
+  B.ks = 1;
+  if (K % 16 == 0) mi::int8_bwd_plan(B);
+  return parts_bytes(B) + rows_bytes(B) + (B.ks > 1 ? (int64_t)B.ks * M * K * 4 : 0);
 }
 
 int backward(mi::Int8GradParams& G, mi::Int8BwdParams& B, int64_t M, int64_t N, int64_t K, int dtype,
@@ -114,25 +130,31 @@ int backward(mi::Int8GradParams& G, mi::Int8BwdParams& B, int64_t M, int64_t N, 
   const int type = float_type(dtype);
   if (type < 0) return report_error(MI_ERR_UNSUPPORTED, "dtype not supported (bfloat16, float16, float32)");
   if (M == 0 || K == 0) return MI_OK;
-  if (((M + 63) / 64) * ((K + 63) / 64) > kMaxTiles || M * N > kMaxArea)
-    return report_error(MI_ERR_UNSUPPORTED, "M * K or M * N too large for one call");
+  if (!backward_fits(M, N, K))
+    return report_error(MI_ERR_UNSUPPORTED, "M * K or the rows too large for one call");
   if (!G.dy || !G.sw || !B.dx || !B.w[0] || (banks == 2 && (!G.gate || !G.up || !G.sw2 || !B.w[1])))
     return bad("null tensor pointer");
   if (!G.dgate != !G.dup) return bad("dgate and dup go together");
-  if (int rc = check_workspace(ws, ws_bytes, backward_need(M, N, banks, type))) return rc;
+  if (int rc = check_workspace(ws, ws_bytes, backward_need(B, M, N, K, banks, type))) return rc;
   G.a = (uint16_t*)ws;
-  G.banks = B.banks = banks;
-  G.terms = B.terms = type + 1;
-  G.np = B.np = (int)np_of(N);
-  G.M = B.M = (int)M;
-  G.N = B.N = (int)N;
-  B.K = (int)K;
-  G.type = B.type = type;
+  G.row = (float*)((char*)ws + parts_bytes(B));
   B.a = G.a;
-  B.splits = 1;
+  B.row = G.row;
+  B.part = (float*)((char*)G.row + rows_bytes(B));
+  G.banks = banks;
+  G.terms = B.terms;
+  G.np = B.np;
+  G.M = B.M;
+  G.N = B.N;
+  G.type = type;
+  G.vec = N % (type == mi::kF32 ? 4 : 8) == 0 && aligned(G.dy, 16) && aligned(G.gate, 16) && aligned(G.up, 16) &&
+          aligned(G.dgate, 16) && aligned(G.dup, 16) && aligned(G.sw, 16) && aligned(G.sw2, 16);
+  B.vec = K % 4 == 0 && aligned(B.dx, type == mi::kF32 ? 16 : 8);
   const hipError_t e = mi::launch_int8_grad(G, s);
   if (e != hipSuccess) return hip_status(e, "int8 gradient launch");
-  return hip_status(mi::launch_int8_bwd_any(B, s), "int8 backward launch");
+  return hip_status(mi::int8_bwd_supported(K, B.w[0], B.w[1]) ? mi::launch_int8_bwd(B, s)
+                                                              : mi::launch_int8_bwd_any(B, s),
+                    "int8 backward launch");
 }
 
 }  // namespace
@@ -164,9 +186,10 @@ int64_t mi_int8_forward_workspace(int64_t M, int64_t N, int64_t K, int banks, in
 int64_t mi_int8_backward_workspace(int64_t M, int64_t N, int64_t K, int banks, int dtype) {
   const int type = float_type(dtype);
   if (M < 0 || N < 0 || K < 0 || banks < 1 || banks > 2 || type < 0 || M > kMaxDim || N > kMaxDim ||
-      M * N > kMaxArea)
+      K > kMaxDim || !backward_fits(M, N, K))
     return -1;
-  return backward_need(M, N, banks, type);
+  mi::Int8BwdParams B{};
+  return backward_need(B, M, N, K, banks, type);
 }
 
 int mi_int8_matmul(void* y, const void* x, const float* x_scales, const int8_t* w,

@@ -38,17 +38,20 @@ struct Int8Params {
   bool vec;  // y, gate, up, part rows of four columns on one store (N and pointers)
 };
 
-// dx[m,k] = sum over banks and n of a[m,n] w[n,k], a split into `terms` bf16 parts:
-// part [(bank * terms + t)][M][np] holds part t of a (zero from n = N on).
+// dx[m,k] = row[m] * sum over banks, parts and n of a[m,n] w[n,k]: the scaled gradients a as fp16,
+// each row times a power of two (1 / row[m]) that puts its largest value into 2^14 .. 2^15, in
+// `terms` parts that add up: [(bank * terms + t)][M][np], zero from n = N on.
 struct Int8BwdParams {
   const uint16_t* a;
+  const float* row;    // [M]
   const int8_t* w[2];  // [N, K]
   void* dx;            // [M, K]
-  float* part;         // splits > 1: fp32 partials [splits][M][K]
+  float* part;         // ks > 1: fp32 sums [ks][M][K]
   int banks, terms, np;
   int M, N, K;
   int type;
-  int splits;
+  int bm, ks, sps;  // int8_bwd.hip: rows of a tile, ranges of sps 64-value steps over the parts
+  bool vec;
 };
 
 // a = dy * sw[n] (one bank), or the two products of the SwiGLU gradient with sw / sw2.
@@ -61,9 +64,11 @@ struct Int8GradParams {
   void* dgate;  // nullable
   void* dup;
   uint16_t* a;
+  float* row;
   int banks, terms, np;
   int M, N;
   int type;
+  bool vec;  // rows and scales on 16 bytes, N a multiple of 8 (fp32: 4)
 };
 
 hipError_t launch_int8_quantize(int8_t* q, float* s, const void* x, int64_t rows, int64_t K,
@@ -74,6 +79,9 @@ void int8_gemm_plan(Int8Params& P);  // from M, N, K and banks: bm, ks, sps
 hipError_t launch_int8_gemm(const Int8Params& P, hipStream_t s);
 hipError_t launch_int8_any(const Int8Params& P, hipStream_t s);
 hipError_t launch_int8_grad(const Int8GradParams& P, hipStream_t s);
+bool int8_bwd_supported(int64_t K, const void* w, const void* w2);
+void int8_bwd_plan(Int8BwdParams& P);  // from M, K, np, banks and terms: bm, ks, sps
+hipError_t launch_int8_bwd(const Int8BwdParams& P, hipStream_t s);
 hipError_t launch_int8_bwd_any(const Int8BwdParams& P, hipStream_t s);
 
 namespace i8 {
@@ -101,6 +109,14 @@ MI_DEV void store_f(void* p, int64_t i, float v) {
 MI_DEV i32x4_t mfma_i8(u32x4_t a, u32x4_t b, i32x4_t c) {
   return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, a),
                                                __builtin_bit_cast(i32x4_t, b), c, 0, 0, 0);
+}
+
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+
+MI_DEV f32x4_t mfma_f16(u32x4_t a, u32x4_t b, f32x4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a),
+                                                __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
 }
 
 // 1 / (1 + e^-g): e^-g overflows to infinity for g < -88, which gives 0, the limit.

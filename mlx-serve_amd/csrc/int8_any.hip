@@ -69,8 +69,8 @@ __global__ void __launch_bounds__(256) int8_any_kernel(Int8Params P) {
 }
 
 // dx: 64 rows x 64 codes of the weight rows' K; 32 values of n a step. The weights' tile is
-// turned in LDS (row k, values n) as exact bf16.
-constexpr int kLdB = 40;  // bf16 values of a staged row
+// turned in LDS (row k, values n) as exact fp16.
+constexpr int kLdB = 40;  // fp16 values of a staged row
 
 template <int T>
 __global__ void __launch_bounds__(256) int8_bwd_any_kernel(Int8BwdParams P) {
@@ -97,16 +97,14 @@ __global__ void __launch_bounds__(256) int8_bwd_any_kernel(Int8BwdParams P) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int k = k0 + wc + j;
-        const float f = on && k < P.K ? (float)w[(int64_t)(n + wr) * P.K + k] : 0.f;
-        bs[(wc + j) * kLdB + wr] = (uint16_t)(__float_as_uint(f) >> 16);
+        const _Float16 f = on && k < P.K ? (_Float16)(float)w[(int64_t)(n + wr) * P.K + k] : (_Float16)0.f;
+        bs[(wc + j) * kLdB + wr] = __builtin_bit_cast(uint16_t, f);
       }
       __syncthreads();
       const u32x4_t b = *reinterpret_cast<const u32x4_t*>(bs + (16 * wave + fr) * kLdB + 8 * q);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        acc[i] = mfma16x16x32(
-            as_bf16x8(b), as_bf16x8(*reinterpret_cast<const u32x4_t*>(as + (16 * i + fr) * kLdB + 8 * q)),
-            acc[i]);
+        acc[i] = mfma_f16(b, *reinterpret_cast<const u32x4_t*>(as + (16 * i + fr) * kLdB + 8 * q), acc[i]);
       __syncthreads();
     }
   }
@@ -114,10 +112,11 @@ __global__ void __launch_bounds__(256) int8_bwd_any_kernel(Int8BwdParams P) {
   for (int i = 0; i < 4; ++i) {
     const int64_t m = m0 + 16 * i + fr;
     if (m >= P.M) continue;
+    const float r = P.row[m];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int k = k0 + 16 * wave + 4 * q + j;
-      if (k < P.K) store_f<T>(P.dx, m * P.K + k, acc[i][j]);
+      if (k < P.K) store_f<T>(P.dx, m * P.K + k, acc[i][j] * r);
     }
   }
 }

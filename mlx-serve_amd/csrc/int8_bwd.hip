@@ -1,0 +1,308 @@
+// The gradient of an int8 product to its activations, on the matrix cores:
+//   dx[m,k] = row[m] * sum over n of a[m,n] w[n,k]
+// with the scaled gradients a in fp16 parts (int8_quant.hip) and the codes as exact fp16, fp32
+// sums; the banks and parts follow one another along the sum.
+//
+// Block: 8 waves as 2 (rows of a) x 4 (columns of w), BM x BN outputs, v_mfma_f32_16x16x32_f16 with
+// D[k][m] = w[n][k] a[m][n]. A step is 64 values of n: rows of a are one cache line, the codes 64
+// rows of BN bytes, both moved by LDS DMA into a ring of R stages as in int8_gemm.hip (one barrier a
+// step, in its middle; the L2 asked for lines ahead). The sum runs along the rows of w, so a
+// fragment takes one column of eight rows: ds_read_b64_tr_b8 gives lane l of 16 column l % 16 of the
+// 8 x 16 bytes that the 16 lanes point at, so w is read as it lies in memory, and no turned copy of
+// it is made. Codes become fp16 in registers, five operations for four: u = code + 128 in the low
+// byte of 0x64 is 1024 + u, minus 1152.
+#include <algorithm>
+#include <atomic>
+
+#include "int8_stage.h"
+#include "prefill_tiles.h"
+
+namespace mi {
+namespace {
+
+using namespace i8;
+
+constexpr int kBN_ = 64;  // values of n a step
+typedef int32_t i32x2_t __attribute__((ext_vector_type(2)));
+
+template <int BM, int BN, int R>
+constexpr int lds_bytes() { return R * (BM * 128 + kBN_ * BN) + 2048; }
+
+// Swizzle of the 16-byte slots of a row of codes. A pass of 32 lanes reads one slot of 16 rows:
+// rows 8e .. 8e+7 of quarters q and q + 1 (n = 16 q + 8 e + j): j and the parity of q tell them
+// apart, and where a row is 128 bytes its lowest bit already does.
+template <int BN>
+MI_DEV int nswz(int n) {
+  return BN == 256 ? (n & 7) | ((n >> 1) & 8) : ((n >> 1) & 3) | ((n >> 2) & 4);
+}
+
+// four codes -> fp16, in order
+MI_DEV u32x2_t codes_f16(uint32_t w) {
+  const uint32_t u = w ^ 0x80808080u, c = 0x64646464u;
+  const f16x2_t off = {(_Float16)-1152.f, (_Float16)-1152.f};
+  const f16x2_t a = __builtin_bit_cast(f16x2_t, perm_b32(c, u, 0x04010400u)) + off;
+  const f16x2_t b = __builtin_bit_cast(f16x2_t, perm_b32(c, u, 0x04030402u)) + off;
+  return u32x2_t{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
+}
+
+MI_DEV i32x2_t read_tr8(const unsigned char* p) {
+  return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2_t*)p);
+}
+
+template <int BM, int BN, int R, bool SPLIT>
+__global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
+int8_bwd_kernel(Int8BwdParams P) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  constexpr int MT = BM / 32, NT = BN / 64;   // 16-row / 16-column tiles of a wave
+  constexpr int XI = BM / 64, WI = BN / 128;  // DMA instructions of a wave a step
+  constexpr int kStage = BM * 128 + kBN_ * BN, kW = BM * 128;
+  constexpr int kRI = 1024 / BN;              // rows of w an instruction moves
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave >> 2, wn = wave & 3;
+  const int fr = lane & 15, q = lane >> 4;
+  const int M = P.M, N = P.N, K = P.K, np = P.np;
+  const int mtiles = (M + BM - 1) / BM;
+  const TileOf at = tile_of_block(mtiles, (K + BN - 1) / BN);
+  const int m0 = at.mt * BM, k0 = at.nt * BN, s0 = at.split * P.sps;
+  const int seg_steps = np / kBN_;
+  const int ns = min(P.sps, P.banks * P.terms * seg_steps - s0);
+  const int mrows = min(BM, M - m0);
+  const int abytes = mrows * np * 2;
+
+  uint32_t xo[XI], wo[WI];
+  int wr[WI];
+#pragma unroll
+  for (int i = 0; i < XI; ++i) {
+    const int r = 8 * (wave * XI + i) + (lane >> 3);
+    xo[i] = (uint32_t)(min(r, mrows - 1) * np * 2 + 16 * ((lane & 7) ^ xswz(r)));
+  }
+#pragma unroll
+  for (int i = 0; i < WI; ++i) {
+    wr[i] = kRI * (wave * WI + i) + lane / (BN / 16);
+    const int c = 16 * ((lane % (BN / 16)) ^ nswz<BN>(wr[i]));
+    wo[i] = k0 + c < K ? (uint32_t)wr[i] * (uint32_t)K + (uint32_t)(k0 + c) : kOOB;
+  }
+  // where a stage reads: part `seg`, values n .. n + 63 of it
+  struct Cursor {
+    int st, seg, n;
+  };
+  auto start = [&](int st) {
+    const int g = s0 + st;
+    return Cursor{st, g / seg_steps, g % seg_steps * kBN_};
+  };
+  auto step = [&](Cursor& c) __attribute__((always_inline)) {
+    ++c.st;
+    c.n += kBN_;
+    if (c.n >= np) {
+      c.n = 0;
+      ++c.seg;
+    }
+  };
+  auto abase = [&](const Cursor& c) { return P.a + ((size_t)c.seg * M + m0) * np; };
+  auto wbase = [&](const Cursor& c) { return P.w[c.seg >= P.terms] + (size_t)c.n * K; };
+  // stages past the range load through resources of zero records (zeros, no traffic), rows from N
+  // on and columns from K on out of bounds
+  auto issue = [&](const Cursor& c, int slot) __attribute__((always_inline)) {
+    const bool on = c.st < ns;
+    const int rows = min(kBN_, N - c.n);
+    unsigned char* b = smem + slot * kStage;
+#pragma unroll
+    for (int i = 0; i < XI; ++i)
+      dma16(rsrc(abase(c), on ? abytes : 0), b + (wave * XI + i) * 1024, xo[i], c.n * 2);
+#pragma unroll
+    for (int i = 0; i < WI; ++i)
+      dma16(rsrc(wbase(c), on ? rows * K : 0), b + kW + (wave * WI + i) * 1024, wr[i] < rows ? wo[i] : kOOB, 0);
+  };
+  // L2 prefetch: waves 0-3 the rows of a, 64 a wave; waves 4, 5 the two lines of the rows of w
+  const int h = min(4, mtiles - at.mt / 4 * 4);
+  const bool pw = wave >= 4;
+  const int pr = (wave & 3) * 64 + lane, pc = (wave & 3) * 128;
+  const bool mine = pw ? pc < BN && k0 + pc < K && at.mt % h == (lane & 3) % h
+                       : pr < mrows && (at.nt & 3) == (wave & 3);
+  const uint32_t po = !mine ? kOOB : pw ? (uint32_t)lane * (uint32_t)K + (uint32_t)(k0 + pc) : (uint32_t)(pr * np * 2);
+  auto prefetch = [&](const Cursor& c) __attribute__((always_inline)) {
+    const bool on = c.st < ns;
+    const int rows = min(kBN_, N - c.n);
+    if (pw)
+      dma4(rsrc(wbase(c), on ? rows * K : 0), smem + R * kStage + wave * 256, lane < rows ? po : kOOB, 0);
+    else
+      dma4(rsrc(abase(c), on ? abytes : 0), smem + R * kStage + wave * 256, po, c.n * 2);
+  };
+
+  f32x4_t acc[NT][MT];
+#pragma unroll
+  for (int a = 0; a < NT; ++a)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[a][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  u32x4_t X[2][MT];
+  i32x2_t A[2][NT];
+  // half e: values n = 16 q + 8 e .. + 7 of both operands (slot 2q + e of a row of a)
+  const int fo0 = fr * 128 + (((2 * q) ^ xswz(fr)) << 4), fo1 = fr * 128 + (((2 * q + 1) ^ xswz(fr)) << 4);
+  const int xr = 16 * wm * MT * 128;
+  const int nr = 16 * q + (fr >> 1);  // row of w in half 0; half 1 is 8 rows on, same swizzle
+  int ao[NT];
+#pragma unroll
+  for (int a = 0; a < NT; ++a) ao[a] = kW + nr * BN + (((wn * NT + a) ^ nswz<BN>(nr)) << 4) + 8 * (fr & 1);
+  auto frags = [&](int slot, int e) __attribute__((always_inline)) {
+    const unsigned char* b = smem + slot * kStage;
+#pragma unroll
+    for (int a = 0; a < NT; ++a) A[e][a] = read_tr8(b + ao[a] + e * 8 * BN);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+      X[e][i] = *reinterpret_cast<const u32x4_t*>(b + xr + (e ? fo1 : fo0) + 16 * i * 128);
+  };
+  auto products = [&](int e) __attribute__((always_inline)) {
+#pragma unroll
+    for (int a = 0; a < NT; ++a) {
+      const u32x2_t lo = codes_f16((uint32_t)A[e][a].x), hi = codes_f16((uint32_t)A[e][a].y);
+      const u32x4_t w = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+      for (int i = 0; i < MT; ++i) acc[a][i] = mfma_f16(w, X[e][i], acc[a][i]);
+    }
+  };
+
+  Cursor ci = start(0), cp = start(R);
+#pragma unroll
+  for (int s = 0; s < R; ++s) {
+    issue(ci, s);
+    prefetch(cp);
+    step(ci);
+    step(cp);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  wait_vm(1 + (R - 1) * (XI + WI + 1));
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  frags(0, 0);
+  int slot = 0;
+#pragma unroll 1
+  for (int t = 0; t < ns; ++t) {
+    const int next = slot + 1 == R ? 0 : slot + 1;
+    frags(slot, 1);
+    products(0);
+#pragma unroll
+    for (int r = 0; r < MT * NT; ++r) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      if (r < MT + NT) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): this wave's reads of stage t
+    wait_vm(1 + (R - 2) * (XI + WI + 1));
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    frags(next, 0);
+    issue(ci, slot);
+    prefetch(cp);
+    step(ci);
+    step(cp);
+    products(1);
+#pragma unroll
+    for (int r = 0; r < MT * NT; ++r) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      if (r < MT + NT) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+      if (r % 2 == 0) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    slot = next;
+  }
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // no DMA may outlive the block
+
+  // acc[a][i] register j is [k = 16 (wn NT + a) + 4q + j][m = 16 (wm MT + i) + fr]
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int m = m0 + 16 * (wm * MT + i) + fr;
+    if (m >= M) continue;
+    const float row = P.row[m];
+#pragma unroll
+    for (int a = 0; a < NT; ++a) {
+      const int k = k0 + 16 * (wn * NT + a) + 4 * q;
+      if (k >= K) continue;  // K is a multiple of 16
+      const f32x4_t v = acc[a][i];
+      if constexpr (SPLIT) {
+        *reinterpret_cast<f32x4_t*>(P.part + ((size_t)at.split * M + m) * K + k) = v;
+      } else {
+        const float o[4] = {v[0] * row, v[1] * row, v[2] * row, v[3] * row};
+        store4(P.dx, (int64_t)m * K + k, P.type, P.vec, 4, o);
+      }
+    }
+  }
+}
+
+// The ranges' sums, added in their order.
+__global__ void __launch_bounds__(256) int8_bwd_reduce_kernel(Int8BwdParams P) {
+  const int64_t mk4 = (int64_t)P.M * P.K / 4, k4 = P.K / 4;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < mk4; i += (int64_t)gridDim.x * 256) {
+    const f32x4_t* p = reinterpret_cast<const f32x4_t*>(P.part) + i;
+    const f32x4_t v = add_splits<8>(p[0], p, mk4, 1, P.ks);
+    const float row = P.row[i / k4];
+    const float o[4] = {v[0] * row, v[1] * row, v[2] * row, v[3] * row};
+    store4(P.dx, 4 * i, P.type, P.vec, 4, o);
+  }
+}
+
+template <int BM, int BN, int R>
+hipError_t launch_tile(const Int8BwdParams& P, hipStream_t s) {
+  constexpr int lds = lds_bytes<BM, BN, R>();
+  static std::atomic<uint64_t> done{0};  // devices whose functions have the attribute
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  const uint64_t bit = (uint64_t)1 << (dev & 63);
+  if (e == hipSuccess && !(done.load() & bit)) {
+    for (auto k : {int8_bwd_kernel<BM, BN, R, false>, int8_bwd_kernel<BM, BN, R, true>})
+      if (e == hipSuccess)
+        e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e == hipSuccess) done |= bit;
+  }
+  if (e != hipSuccess) return e;
+  const dim3 grid((unsigned)(((P.M + BM - 1) / BM) * ((P.K + BN - 1) / BN)), (unsigned)P.ks);
+  if (P.ks > 1)
+    hipLaunchKernelGGL((int8_bwd_kernel<BM, BN, R, true>), grid, dim3(512), lds, s, P);
+  else
+    hipLaunchKernelGGL((int8_bwd_kernel<BM, BN, R, false>), grid, dim3(512), lds, s, P);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+// Rows of codes on 16 bytes.
+bool int8_bwd_supported(int64_t K, const void* w, const void* w2) {
+  return ((uintptr_t)w | (uintptr_t)w2 | (uintptr_t)K) % 16 == 0;
+}
+
+// As int8_gemm_plan.
+void int8_bwd_plan(Int8BwdParams& P) {
+  const int steps = P.banks * P.terms * (P.np / kBN_);
+  struct Tile { int bm, bn; double us; };
+  constexpr Tile kTiles[] = {{256, 256, 1.7}, {128, 256, 1.0}, {64, 128, 0.5}};
+  double best = 1e30;
+  for (const Tile& t : kTiles) {
+    const int64_t tiles = (int64_t)((P.M + t.bm - 1) / t.bm) * ((P.K + t.bn - 1) / t.bn);
+    for (int k = 1; k <= std::max(1, steps / 4) && k <= 64; ++k) {
+      const int sps = (steps + k - 1) / k, ks = (steps + sps - 1) / sps;
+      const double part = ks > 1 ? (double)ks * P.M * P.K * 8 / 5e6 + 4.0 : 0.0;
+      const double cost = (double)((tiles * ks + 255) / 256) * (sps * t.us + 2.0) + part;
+      if (cost < best - 1e-9) {
+        best = cost;
+        P.bm = t.bm;
+        P.ks = ks;
+        P.sps = sps;
+      }
+    }
+  }
+}
+
+hipError_t launch_int8_bwd(const Int8BwdParams& P, hipStream_t s) {
+  const hipError_t e = P.bm == 256   ? launch_tile<256, 256, 3>(P, s)
+                       : P.bm == 128 ? launch_tile<128, 256, 4>(P, s)
+                                     : launch_tile<64, 128, 6>(P, s);
+  if (e != hipSuccess || P.ks == 1) return e;
+  int64_t g = ((int64_t)P.M * P.K / 4 + 255) / 256;
+  if (g > 8192) g = 8192;
+  hipLaunchKernelGGL(int8_bwd_reduce_kernel, dim3((unsigned)g), dim3(256), 0, s, P);
+  return hipGetLastError();
+}
+
+}  // namespace mi

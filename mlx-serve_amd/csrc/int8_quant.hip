@@ -200,88 +200,231 @@ hipError_t launch_type(int8_t* q, float* s, const void* x, int64_t rows, int64_t
 }
 
 // ------------------------------------------------------------- SwiGLU gradient ---
-// Values times their channel scale, in bf16 parts for the matrix product that follows: one part,
-// rounded, for bf16 gradients; for fp16 and fp32 the leading 8 bits, cut off (so that what is
-// left is exact), then the next 8, the last part rounded: 16 and 24 bits in all.
+// The values that the backward product sums, times their channel scale, as fp16: its 11 bits are
+// more than a bf16 gradient has, and all that an fp16 one has; fp32 gradients take a second part
+// for what the first leaves (22 bits). fp16's range is met by a power of two for each row, exact
+// both ways: the row's largest value goes into 2^14 .. 2^15, values down to 2^-28 of it keep
+// their 11 bits, and below that the error is 2^-39 of it. A row with an infinity or a NaN is
+// taken as it is.
+//
+// Memory-bound (three reads, four writes of [M, N] with both outputs); a row is held in
+// registers between its maximum and the parts.
+
+// power of two for a row whose largest magnitude has these bits, and its reciprocal
+MI_DEV void row_power(uint32_t maxbits, float* scale, float* inv) {
+  const int e = (int)(maxbits >> 23);
+  const int b = e == 255 || maxbits == 0 ? 127 : min(268 - e, 253);
+  *scale = __uint_as_float((uint32_t)b << 23);
+  *inv = __uint_as_float((uint32_t)(254 - b) << 23);
+}
+
 template <int TERMS>
-MI_DEV void split_bf16(float v, uint16_t (&p)[TERMS]) {
-  if constexpr (TERMS == 1) {
-    p[0] = (uint16_t)f32_to_bf16_bits(v);
+MI_DEV void parts_of(float v, uint16_t (&p)[TERMS]) {
+  const _Float16 hi = (_Float16)v;
+  p[0] = __builtin_bit_cast(uint16_t, hi);
+  if constexpr (TERMS == 2) {
+    const float f = (float)hi;
+    const bool fin = (__float_as_uint(f) & 0x7F800000u) != 0x7F800000u;
+    p[1] = __builtin_bit_cast(uint16_t, (_Float16)(fin ? v - f : 0.f));
+  }
+}
+
+template <int T>
+struct Grad {
+  float a, b, dg, du;
+};
+template <int T, int BANKS>
+MI_DEV Grad<T> gradient(float dy, float g, float u, float sw, float sw2) {
+  Grad<T> r;
+  if constexpr (BANKS == 1) {
+    r.a = dy * sw;
+    r.b = r.dg = r.du = 0.f;
   } else {
-    const bool fin = (__float_as_uint(v) & 0x7F800000u) != 0x7F800000u;
-    float r = v;
+    const float sig = sigmoid_f(g);
+    r.dg = dy * u * sig * (1.f + g * (1.f - sig));
+    r.du = dy * g * sig;
+    r.a = r.dg * sw;
+    r.b = r.du * sw2;
+  }
+  return r;
+}
+MI_DEV uint32_t mag(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+
+// values of a 16-byte vector
+template <int T, int E>
+MI_DEV void unpack(const void* p, int64_t v, float (&f)[E]) {
+  const u32x4_t x = reinterpret_cast<const u32x4_t*>(p)[v];
 #pragma unroll
-    for (int t = 0; t < TERMS; ++t) {
-      const bool last = t == TERMS - 1;
-      p[t] = last || !fin ? (uint16_t)f32_to_bf16_bits(r) : (uint16_t)(__float_as_uint(r) >> 16);
-      r = fin ? r - bf16_bits_to_f32(p[t]) : 0.f;
+  for (int j = 0; j < E; ++j) {
+    if constexpr (T == kF32) {
+      f[j] = __uint_as_float(x[j]);
+    } else {
+      const uint16_t h = (uint16_t)(x[j / 2] >> (16 * (j & 1)));
+      f[j] = T == kBF16 ? bf16_bits_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
+    }
+  }
+}
+template <int E>
+MI_DEV void unpack_f32(const float* p, int n, float (&f)[E]) {
+#pragma unroll
+  for (int j = 0; j < E; j += 4) {
+    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(p + n + j);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f[j + k] = x[k];
+  }
+}
+template <int T, int E>
+MI_DEV void pack_store(void* p, int64_t v, const float (&f)[E]) {
+  u32x4_t o = {0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    if constexpr (T == kF32)
+      o[j] = __float_as_uint(f[j]);
+    else
+      o[j / 2] |= (T == kBF16 ? f32_to_bf16_bits(f[j])
+                              : (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[j])) << (16 * (j & 1));
+  }
+  reinterpret_cast<u32x4_t*>(p)[v] = o;
+}
+
+// A block a row, VPT vectors of 16 bytes a thread; np / E vectors of `a` a row.
+template <int T, int BANKS, int WPR, int VPT>
+__global__ void __launch_bounds__(WPR * 64) int8_grad_kernel(Int8GradParams P) {
+  constexpr int E = T == kF32 ? 4 : 8, TERMS = T == kF32 ? 2 : 1;
+  __shared__ uint32_t part[WPR];
+  const int64_t m = blockIdx.x;
+  const int nv = P.N / E, npv = P.np / E;
+  float a[VPT][E], b[BANKS == 2 ? VPT : 1][E];
+  uint32_t mx = 0;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int c = threadIdx.x + i * WPR * 64;
+    const bool on = c < nv;
+    float dy[E], g[E], u[E], sw[E], sw2[E], dg[E], du[E];
+    if (on) {
+      unpack<T, E>(P.dy, m * nv + c, dy);
+      unpack_f32<E>(P.sw, c * E, sw);
+      if constexpr (BANKS == 2) {
+        unpack<T, E>(P.gate, m * nv + c, g);
+        unpack<T, E>(P.up, m * nv + c, u);
+        unpack_f32<E>(P.sw2, c * E, sw2);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      a[i][j] = 0.f;
+      if constexpr (BANKS == 2) b[i][j] = 0.f;
+      if (on) {
+        const Grad<T> r = gradient<T, BANKS>(dy[j], BANKS == 2 ? g[j] : 0.f, BANKS == 2 ? u[j] : 0.f,
+                                             sw[j], BANKS == 2 ? sw2[j] : 0.f);
+        a[i][j] = r.a;
+        mx = max(mx, mag(r.a));
+        if constexpr (BANKS == 2) {
+          b[i][j] = r.b;
+          mx = max(mx, mag(r.b));
+        }
+        dg[j] = r.dg;
+        du[j] = r.du;
+      }
+    }
+    if (BANKS == 2 && on && P.dgate) {
+      pack_store<T, E>(P.dgate, m * nv + c, dg);
+      pack_store<T, E>(P.dup, m * nv + c, du);
+    }
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, d));
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = mx;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < WPR; ++i) mx = max(mx, part[i]);
+  float scale, inv;
+  row_power(mx, &scale, &inv);
+  if (threadIdx.x == 0) P.row[m] = inv;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int c = threadIdx.x + i * WPR * 64;
+    if (c >= npv) continue;
+#pragma unroll
+    for (int k = 0; k < BANKS; ++k) {
+      uint16_t p[E][TERMS];
+#pragma unroll
+      for (int j = 0; j < E; ++j) parts_of<TERMS>((k ? b[BANKS == 2 ? i : 0][j] : a[i][j]) * scale, p[j]);
+#pragma unroll
+      for (int t = 0; t < TERMS; ++t) {
+        uint32_t o[E / 2];
+#pragma unroll
+        for (int j = 0; j < E; j += 2) o[j / 2] = p[j][t] | (uint32_t)p[j + 1][t] << 16;
+        uint16_t* q = P.a + ((int64_t)(k * TERMS + t) * P.M + m) * P.np + c * E;
+        if constexpr (E == 8)
+          *reinterpret_cast<u32x4_t*>(q) = u32x4_t{o[0], o[1], o[E / 2 - 2], o[E / 2 - 1]};
+        else
+          *reinterpret_cast<u32x2_t*>(q) = u32x2_t{o[0], o[1]};
+      }
     }
   }
 }
 
-template <int T, int BANKS, int VEC>
-__global__ void __launch_bounds__(256) int8_grad_kernel(Int8GradParams P) {
-  constexpr int TERMS = T + 1;
-  const int np = P.np, N = P.N;
-  const int64_t per_row = np / VEC, total = per_row * P.M;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t m = i / per_row;
-    const int n0 = (int)(i - m * per_row) * VEC;
-    const int64_t at = m * N + n0;
-    const bool on = n0 < N;  // VEC > 1 only where N is a multiple of it
-    uint16_t part[BANKS][TERMS][VEC];
-    float dg[VEC], du[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      float a = 0.f, b = 0.f;
-      dg[j] = du[j] = 0.f;
-      if (on) {
-        const float dy = load_f<T>(P.dy, at + j);
-        if constexpr (BANKS == 1) {
-          a = dy * P.sw[n0 + j];
-        } else {
-          const float g = load_f<T>(P.gate, at + j), u = load_f<T>(P.up, at + j);
-          const float sig = sigmoid_f(g);
-          dg[j] = dy * u * sig * (1.f + g * (1.f - sig));
-          du[j] = dy * g * sig;
-          a = dg[j] * P.sw[n0 + j];
-          b = du[j] * P.sw2[n0 + j];
-        }
-      }
-      uint16_t p[TERMS];
-      split_bf16<TERMS>(a, p);
-#pragma unroll
-      for (int t = 0; t < TERMS; ++t) part[0][t][j] = p[t];
-      if constexpr (BANKS == 2) {
-        split_bf16<TERMS>(b, p);
-#pragma unroll
-        for (int t = 0; t < TERMS; ++t) part[1][t][j] = p[t];
+// Any width and alignment: a block a row, which is read and computed twice.
+template <int T, int BANKS>
+__global__ void __launch_bounds__(256) int8_grad_any_kernel(Int8GradParams P) {
+  constexpr int TERMS = T == kF32 ? 2 : 1;
+  __shared__ uint32_t part[4];
+  for (int64_t m = blockIdx.x; m < P.M; m += gridDim.x) {
+    const int64_t at = m * P.N;
+    auto grad = [&](int n) {
+      return gradient<T, BANKS>(load_f<T>(P.dy, at + n), BANKS == 2 ? load_f<T>(P.gate, at + n) : 0.f,
+                                BANKS == 2 ? load_f<T>(P.up, at + n) : 0.f, P.sw[n], BANKS == 2 ? P.sw2[n] : 0.f);
+    };
+    uint32_t mx = 0;
+    for (int n = threadIdx.x; n < P.N; n += 256) {
+      const Grad<T> r = grad(n);
+      mx = max(mx, max(mag(r.a), mag(r.b)));
+      if (BANKS == 2 && P.dgate) {
+        store_f<T>(P.dgate, at + n, r.dg);
+        store_f<T>(P.dup, at + n, r.du);
       }
     }
+    for (int d = 32; d; d >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, d));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = mx;
+    __syncthreads();
+    mx = max(max(part[0], part[1]), max(part[2], part[3]));
+    float scale, inv;
+    row_power(mx, &scale, &inv);
+    if (threadIdx.x == 0) P.row[m] = inv;
+    for (int n = threadIdx.x; n < P.np; n += 256) {
+      Grad<T> r = {0.f, 0.f, 0.f, 0.f};
+      if (n < P.N) r = grad(n);
 #pragma unroll
-    for (int b = 0; b < BANKS; ++b)
+      for (int k = 0; k < BANKS; ++k) {
+        uint16_t p[TERMS];
+        parts_of<TERMS>((k ? r.b : r.a) * scale, p);
 #pragma unroll
-      for (int t = 0; t < TERMS; ++t) {
-        uint16_t* o = P.a + ((int64_t)(b * TERMS + t) * P.M + m) * np + n0;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) o[j] = part[b][t][j];
-      }
-    if (BANKS == 2 && on && P.dgate) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        store_f<T>(P.dgate, at + j, dg[j]);
-        store_f<T>(P.dup, at + j, du[j]);
+        for (int t = 0; t < TERMS; ++t) P.a[((int64_t)(k * TERMS + t) * P.M + m) * P.np + n] = p[t];
       }
     }
   }
+}
+
+template <int T, int BANKS, int WPR, int VPT>
+hipError_t launch_grad_rows(const Int8GradParams& P, hipStream_t s) {
+  hipLaunchKernelGGL((int8_grad_kernel<T, BANKS, WPR, VPT>), dim3((unsigned)P.M), dim3(WPR * 64), 0, s, P);
+  return hipGetLastError();
 }
 
 template <int T, int BANKS>
 hipError_t launch_grad(const Int8GradParams& P, hipStream_t s) {
-  const int64_t total = (int64_t)P.M * P.np;
-  int64_t g = (total + 255) / 256;
-  if (g > 16384) g = 16384;
-  hipLaunchKernelGGL((int8_grad_kernel<T, BANKS, 1>), dim3((unsigned)g), dim3(256), 0, s, P);
+  const int npv = P.np / (T == kF32 ? 4 : 8);
+  if (P.vec && npv <= 4096 && P.M <= 1 << 21) {  // (below 2^32 threads)
+    if (npv <= 256) return launch_grad_rows<T, BANKS, 4, 1>(P, s);
+    if (npv <= 512) return launch_grad_rows<T, BANKS, 4, 2>(P, s);
+    if (npv <= 1024) return launch_grad_rows<T, BANKS, 16, 1>(P, s);
+    if (npv <= 2048) return launch_grad_rows<T, BANKS, 16, 2>(P, s);
+    return launch_grad_rows<T, BANKS, 16, 4>(P, s);
+  }
+  hipLaunchKernelGGL((int8_grad_any_kernel<T, BANKS>), dim3((unsigned)(P.M < 65536 ? P.M : 65536)), dim3(256), 0,
+                     s, P);
   return hipGetLastError();
 }
 

@@ -1,0 +1,43 @@
+// Staging helpers of the int8 matrix kernels: buffer loads into LDS, waits, the row swizzle.
+#pragma once
+#include "int8.h"
+#include "qmv_common.h"
+
+namespace mi {
+namespace i8 {
+
+using qmv_detail::vmcnt_imm;
+
+constexpr int kBufFlags = 0x00020000;   // raw dword access
+constexpr uint32_t kOOB = 0x7FFFFFF0u;  // past any resource: the load returns 0
+// XOR swizzle of the 16-byte slots of a 128-byte row. A ds_read_b128 pass serves lanes 0-3, 12-15,
+// 20-23 and 24-27 of a half together: rows 0-3 and 12-15 of quarter q, 4-11 of quarter q + 1.
+// With slots 2q + e these keep apart.
+MI_DEV int xswz(int r) { return (r & 2) | ((r >> 2) & 1) | ((r >> 1) & 4); }
+
+MI_DEV void dma16(__amdgpu_buffer_rsrc_t rs, unsigned char* lds, uint32_t voff, int soff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)lds, 16,
+                                           voff, soff, 0, 0);
+}
+MI_DEV void dma4(__amdgpu_buffer_rsrc_t rs, unsigned char* lds, uint32_t voff, int soff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)lds, 4,
+                                           voff, soff, 0, 0);
+}
+MI_DEV __amdgpu_buffer_rsrc_t rsrc(const void* p, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, bytes, kBufFlags);
+}
+
+// s_waitcnt vmcnt(n); n is a constant after inlining
+MI_DEV void wait_vm(int n) {
+  switch (n) {
+#define C(n) case n: __builtin_amdgcn_s_waitcnt(vmcnt_imm(n)); break;
+    C(1) C(2) C(3) C(4) C(5) C(6) C(7) C(8) C(9) C(10) C(11) C(12) C(13) C(14) C(15) C(16) C(17)
+    C(18) C(19) C(20) C(21) C(22) C(23) C(24) C(25) C(26) C(27) C(28)
+    default: __builtin_amdgcn_s_waitcnt(vmcnt_imm(0)); break;
+#undef C
+  }
+}
+
+
+}  // namespace i8
+}  // namespace mi

@@ -7,8 +7,11 @@ import torch
 U = 2.0 ** -24
 HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
 FLOOR = {torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -150}
-# bf16 parts of a scaled gradient: what they leave of it
-PARTS = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -16, torch.float32: 2.0 ** -24}
+# fp16 parts of a scaled gradient and what they leave of it: half a step of 11 bits, and of what one
+# part leaves where there are two. A row is scaled so that its largest value is 2^14 at least, and
+# half of fp16's smallest subnormal, 2^-25, is then 2^-39 of that largest value.
+PARTS = {torch.bfloat16: (1, 2.0 ** -11), torch.float16: (1, 2.0 ** -11), torch.float32: (2, 2.0 ** -22)}
+SMALL = 2.0 ** -39
 
 
 def quantize(x):
@@ -70,29 +73,37 @@ def grads(dy, g, u):
     return dg, du, 1.01 * tg + (dy * u).abs() * tiny, 1.01 * tu + (dy * g).abs() * tiny
 
 
-def through(a, ta, w, sw, t):
+def through(a, ta, w, sw, t, top):
     """(sum_n a[m,n] sw[n] w[n,k], its tolerance before the output's rounding): the scaled value rounds
-    once in fp32 and is cut to its bf16 parts; a sum of n terms is off by at most n steps (2 U) of the
-    sum of their magnitudes, parts counted as terms."""
+    once in fp32 and is cut to its fp16 parts (`top`: the row's largest); a sum of n terms is off by at
+    most n steps (2 U) of the sum of their magnitudes, parts counted as terms, and the row's power of
+    two is exact."""
     b = a * sw.double()[None, :]
     wd = w.double()
-    n = a.shape[1] * {torch.bfloat16: 1, torch.float16: 2, torch.float32: 3}[t]
+    parts, left = PARTS[t]
+    n = a.shape[1] * parts
     mag = b.abs() @ wd.abs()
-    err = (ta * sw.double()[None, :].abs()) @ wd.abs()
-    return b @ wd, 1.01 * (mag * (PARTS[t] + U + 2 * U * n) + err)
+    err = (ta * sw.double()[None, :].abs()) @ wd.abs() + SMALL * top[:, None] * wd.abs().sum(0)
+    return b @ wd, 1.01 * (mag * (left + U + 2 * U * n) + err)
+
+
+def _top(*scaled):
+    return torch.stack([v.abs().amax(1) for v in scaled]).amax(0)
 
 
 def matmul_backward(dy, w, sw):
     t = dy.dtype
-    dx, tol = through(dy.double(), torch.zeros_like(dy, dtype=torch.float64), w, sw, t)
+    dx, tol = through(dy.double(), torch.zeros_like(dy, dtype=torch.float64), w, sw, t, _top(dy.double() * sw.double()))
     return dx, 1.01 * HALF[t] * dx.abs() + tol + FLOOR[t]
 
 
 def gate_up_backward(dy, g, u, wg, sg, wu, su):
     t = dy.dtype
     dg, du, tg, tu = grads(dy, g, u)
-    a, ta = through(dg, tg, wg, sg, t)
-    b, tb = through(du, tu, wu, su, t)
+    top = _top(dg * sg.double(), du * su.double())
+    a, ta = through(dg, tg, wg, sg, t, top)
+    b, tb = through(du, tu, wu, su, t, top)
     dx = a + b
     out = lambda v, e: 1.01 * HALF[t] * v.abs() + e + FLOOR[t]
-    return (dx, dg, du), (out(dx, ta + tb), out(dg, tg), out(du, tu))
+    # (the two banks are one sum of 2 N terms: each bound counts its own N once more)
+    return (dx, dg, du), (out(dx, 2 * (ta + tb)), out(dg, tg), out(du, tu))
