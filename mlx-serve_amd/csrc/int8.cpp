@@ -58,16 +58,33 @@ int64_t codes_bytes(int64_t M, int64_t K) { return up(M * up(K, 16), 256); }
 int64_t quant_bytes(int64_t M, int64_t K, int x_dtype) {
   return x_dtype == MI_DTYPE_INT8 ? 0 : codes_bytes(M, K) + up(M * 4, 256);
 }
+bool fused_token(int64_t M, int64_t K, int x_dtype) {
+  return x_dtype != MI_DTYPE_INT8 && mi::int8_gemv_fuses(M, K, float_type(x_dtype));
+}
 int64_t forward_need(mi::Int8Params& P, int64_t M, int64_t N, int64_t K, int x_dtype) {
-  if (M == 0 || N == 0 || K == 0) return 0;
+  if (M == 0 || N == 0 || K == 0 || fused_token(M, K, x_dtype)) return 0;
   P.M = (int)M;
   P.N = (int)N;
   P.K = (int)K;
   P.ks = 1;
-  if (K % 16 == 0) mi::int8_gemm_plan(P);
+  P.nt = 0;
+  if (K % 16 == 0) {  // up to 16 rows the few-row kernel, up to 64 the one that should be faster
+    const double few = M <= mi::kInt8FewRows ? mi::int8_gemv_plan(P) : 0.0;
+    const int nt = P.nt;
+    const double tiles = M > 16 ? mi::int8_gemm_plan(P) : 0.0;
+    if (nt && M > 16 && tiles < few) P.nt = 0;
+    if (P.nt) P.ks = 1;
+  }
   return quant_bytes(M, K, x_dtype) + (P.ks > 1 ? (int64_t)P.ks * P.banks * M * N * 4 : 0);
 }
+// Blocks of a launch, below 2^32 threads.
+bool forward_fits(int64_t M, int64_t N) {
+  return ((M + 63) / 64) * ((N + 63) / 64) <= kMaxTiles && (M > mi::kInt8FewRows || N <= (int64_t)1 << 26);
+}
 bool aligned(const void* p, int a) { return (uintptr_t)p % a == 0; }
+bool rows_on_16(const mi::Int8Params& P) {
+  return ((uintptr_t)P.x | (uintptr_t)P.ldx | (uintptr_t)P.w | (uintptr_t)P.w2 | (uintptr_t)P.K) % 16 == 0;
+}
 
 int forward(mi::Int8Params& P, const void* x, const float* x_scales, int64_t M, int64_t N,
             int64_t K, int x_dtype, int y_dtype, void* ws, int64_t ws_bytes, hipStream_t s) {
@@ -82,17 +99,26 @@ int forward(mi::Int8Params& P, const void* x, const float* x_scales, int64_t M, 
     return report_error(MI_ERR_UNSUPPORTED, "K over 131071: the int32 sums could overflow");
   if (xt >= 0 && x_scales) return bad("x_scales belong to int8 x");
   if (M == 0 || N == 0) return MI_OK;
-  if (((M + 63) / 64) * ((N + 63) / 64) > kMaxTiles)
-    return report_error(MI_ERR_UNSUPPORTED, "M * N too large for one call");
+  if (!forward_fits(M, N)) return report_error(MI_ERR_UNSUPPORTED, "M * N too large for one call");
   if (!P.y || !x || !P.w || !P.sw || (xt < 0 && !x_scales)) return bad("null tensor pointer");
   P.banks = P.w2 ? 2 : 1;
-  if (int rc = check_workspace(ws, ws_bytes, forward_need(P, M, N, K, x_dtype))) return rc;
+  const int64_t need = forward_need(P, M, N, K, x_dtype);
+  if (int rc = check_workspace(ws, ws_bytes, need)) return rc;
   P.part = (int32_t*)((char*)ws + quant_bytes(M, K, x_dtype));
   const int a4 = P.type == mi::kF32 ? 16 : 8;
   P.vec = N % 4 == 0 && aligned(P.y, a4) && aligned(P.gate, a4) && aligned(P.up, a4);
+  P.M = (int)M;
+  P.N = (int)N;
+  P.K = (int)K;
   P.x = (const int8_t*)x;
   P.sx = x_scales;
   P.ldx = K;
+  if (fused_token(M, K, x_dtype)) {
+    P.xf = x;
+    P.xf_type = xt;
+    return hip_status(rows_on_16(P) ? mi::launch_int8_gemv(P, s) : mi::launch_int8_any(P, s),
+                      "int8 matmul launch");
+  }
   if (xt >= 0) {
     P.ldx = up(K, 16);
     P.x = (const int8_t*)ws;
@@ -100,8 +126,9 @@ int forward(mi::Int8Params& P, const void* x, const float* x_scales, int64_t M, 
     const hipError_t e = mi::launch_int8_quantize((int8_t*)ws, (float*)P.sx, x, M, K, P.ldx, xt, s);
     if (e != hipSuccess) return hip_status(e, "int8 quantize launch");
   }
-  return hip_status(mi::int8_gemm_supported(N, K, P.x, P.ldx, P.w, P.w2) ? mi::launch_int8_gemm(P, s)
-                                                                         : mi::launch_int8_any(P, s),
+  return hip_status(!rows_on_16(P) ? mi::launch_int8_any(P, s)
+                    : P.nt         ? mi::launch_int8_gemv(P, s)
+                                   : mi::launch_int8_gemm(P, s),
                     "int8 matmul launch");
 }
 
@@ -176,7 +203,7 @@ int mi_int8_quantize(int8_t* q, float* scales, const void* x, int64_t rows, int6
 
 int64_t mi_int8_forward_workspace(int64_t M, int64_t N, int64_t K, int banks, int x_dtype) {
   if (M < 0 || N < 0 || K < 0 || banks < 1 || banks > 2 || M > kMaxDim || N > kMaxDim ||
-      K > mi::kInt8MaxK || ((M + 63) / 64) * ((N + 63) / 64) > kMaxTiles)
+      K > mi::kInt8MaxK || !forward_fits(M, N) || (x_dtype != MI_DTYPE_INT8 && float_type(x_dtype) < 0))
     return -1;
   mi::Int8Params P{};
   P.banks = banks;

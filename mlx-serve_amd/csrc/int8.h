@@ -11,6 +11,7 @@ enum FloatType { kBF16 = 0, kF16 = 1, kF32 = 2 };
 
 // The int32 sum of K products of codes is exact up to here: 131071 * 128 * 128 < 2^31.
 constexpr int64_t kInt8MaxK = 131071;
+constexpr int64_t kInt8FewRows = 64;  // rows that int8_gemv.hip can take
 
 // y[m,n] = sx[m] * sw[n] * sum_k x[m,k] w[n,k] (+ bias[n]), or with a second bank (w2)
 // y = silu(g) * u of the two products, which go to `gate` and `up` as well where given.
@@ -35,6 +36,7 @@ struct Int8Params {
   // through int32 sums [ks][banks][M][N] in `part`
   int bm, ks, sps;
   int32_t* part;
+  int nt;    // int8_gemv.hip: 16-row tiles of a wave; 0: another kernel
   bool vec;  // y, gate, up, part rows of four columns on one store (N and pointers)
 };
 
@@ -73,9 +75,10 @@ struct Int8GradParams {
 
 hipError_t launch_int8_quantize(int8_t* q, float* s, const void* x, int64_t rows, int64_t K,
                                 int64_t ldq, int type, hipStream_t st);
-bool int8_gemm_supported(int64_t N, int64_t K, const void* x, int64_t ldx, const void* w,
-                         const void* w2);
-void int8_gemm_plan(Int8Params& P);  // from M, N, K and banks: bm, ks, sps
+double int8_gemv_plan(Int8Params& P);  // nt, from M, N, K and banks; returns estimated us
+bool int8_gemv_fuses(int64_t M, int64_t K, int type);
+hipError_t launch_int8_gemv(const Int8Params& P, hipStream_t s);
+double int8_gemm_plan(Int8Params& P);  // bm, ks, sps, from the same; returns estimated us
 hipError_t launch_int8_gemm(const Int8Params& P, hipStream_t s);
 hipError_t launch_int8_any(const Int8Params& P, hipStream_t s);
 hipError_t launch_int8_grad(const Int8GradParams& P, hipStream_t s);
@@ -101,6 +104,59 @@ MI_DEV void store_f(void* p, int64_t i, float v) {
     ((_Float16*)p)[i] = (_Float16)v;
   else
     ((float*)p)[i] = v;
+}
+
+// Codes of a row: s = max |x| / 127, rounded once, and the integers nearest to x / s (ties to even),
+// exactly: x * (1/s) is within a few units of 2^-24 of the quotient, so its nearest integer q is
+// right unless the quotient lies next to a border, and r = x - q s is exact in one fma (x and s
+// have 24 bits, |r| < s, and both are multiples of s's last bit, or q = 0). So |r| < s/2 proves q,
+// and the rare others are settled from r.
+constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: v + kMagic rounds v to an integer (ties to
+                                      // even), whose two's complement is the sum's low bits
+constexpr float kTiny = 0x1p-100f;    // below, x and s are scaled by 2^100 (exact)
+
+struct RowScale {
+  float s, inv, half;
+  bool fin, tiny;  // codes are 0 unless s is finite and not 0
+};
+
+MI_DEV RowScale row_scale(uint32_t maxbits) {
+  RowScale r;
+  r.s = __uint_as_float(maxbits) / 127.f;
+  r.fin = r.s > 0.f && r.s < __builtin_inff();
+  r.tiny = r.s < kTiny;
+  r.inv = r.fin ? 1.f / (r.tiny ? r.s * 0x1p100f : r.s) : 0.f;
+  r.half = 0.5f * r.s;
+  return r;
+}
+
+// any row and value
+MI_DEV int code_of(float x, const RowScale& R) {
+  if (!R.fin) return 0;
+  const float s = R.tiny ? R.s * 0x1p100f : R.s;
+  if (R.tiny) x *= 0x1p100f;
+  float q = rintf(x * R.inv);
+  const float d = fmaf(-q, s, x);
+  const float away = d > 0.f ? 1.f : -1.f, h = 0.5f * s;
+  if (fabsf(d) > h || (fabsf(d) == h && ((int)q & 1))) q += away;
+  return (int)fminf(fmaxf(q, -127.f), 127.f);
+}
+
+// four codes in a dword
+MI_DEV uint32_t codes4(const float (&x)[4], const RowScale& R) {
+  uint32_t t[4];
+  bool sure = R.fin && !R.tiny;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float v = fmaf(x[i], R.inv, kMagic);
+    t[i] = __float_as_uint(v);
+    sure = sure && fabsf(fmaf(-(v - kMagic), R.s, x[i])) < R.half;
+  }
+  if (!sure) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t[i] = (uint32_t)code_of(x[i], R);
+  }
+  return perm_b32(perm_b32(t[3], t[2], 0x0C0C0400u), perm_b32(t[1], t[0], 0x0C0C0400u), 0x05040100u);
 }
 
 // 16 rows x 64 codes of each operand: lane l holds 16 codes of row l % 16, the quarter l / 16

@@ -68,6 +68,52 @@ __global__ void __launch_bounds__(256) int8_any_kernel(Int8Params P) {
   }
 }
 
+// One float token of sizes that int8_gemv.hip would quantize in its launch, on pointers it cannot
+// take: the same here, with no workspace. A wave has four columns at a time.
+template <int T, bool DUAL>
+__global__ void __launch_bounds__(256) int8_token_any_kernel(Int8Params P) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  uint32_t* part = reinterpret_cast<uint32_t*>(smem);
+  int8_t* xs = reinterpret_cast<int8_t*>(smem + 16);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  uint32_t m = 0;
+  for (int k = tid; k < P.K; k += 256) m = max(m, __float_as_uint(load_f<T>(P.xf, k)) & 0x7FFFFFFFu);
+  for (int d = 32; d; d >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
+  if (lane == 0) part[wave] = m;
+  __syncthreads();
+  const RowScale R = row_scale(max(max(part[0], part[1]), max(part[2], part[3])));
+  for (int k = tid; k < P.K; k += 256) xs[k] = (int8_t)code_of(load_f<T>(P.xf, k), R);
+  __syncthreads();
+  const int n = ((int)blockIdx.x * 4 + wave) * 4;
+  if (n >= P.N) return;
+  int32_t s[2][4] = {};
+  for (int j = 0; j < 4 && n + j < P.N; ++j) {
+    const int64_t row = (int64_t)(n + j) * P.K;
+    for (int k = lane; k < P.K; k += 64) {
+      s[0][j] += (int)xs[k] * (int)P.w[row + k];
+      if constexpr (DUAL) s[1][j] += (int)xs[k] * (int)P.w2[row + k];
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < (DUAL ? 2 : 1); ++b)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      for (int d = 32; d; d >>= 1) s[b][j] += __shfl_xor(s[b][j], d);
+  if (lane == 0)
+    finish4<DUAL>(P, 0, n, i32x4_t{s[0][0], s[0][1], s[0][2], s[0][3]},
+                  i32x4_t{s[1][0], s[1][1], s[1][2], s[1][3]}, R.s, load_cols<DUAL>(P, n));
+}
+
+template <int T>
+hipError_t launch_token(const Int8Params& P, hipStream_t s) {
+  const dim3 grid((unsigned)((P.N + 15) / 16));
+  if (P.w2)
+    hipLaunchKernelGGL((int8_token_any_kernel<T, true>), grid, dim3(256), 16 + P.K, s, P);
+  else
+    hipLaunchKernelGGL((int8_token_any_kernel<T, false>), grid, dim3(256), 16 + P.K, s, P);
+  return hipGetLastError();
+}
+
 // dx: 64 rows x 64 codes of the weight rows' K; 32 values of n a step. The weights' tile is
 // turned in LDS (row k, values n) as exact fp16.
 constexpr int kLdB = 40;  // fp16 values of a staged row
@@ -131,6 +177,10 @@ hipError_t launch_bwd(const Int8BwdParams& P, hipStream_t s) {
 }  // namespace
 
 hipError_t launch_int8_any(const Int8Params& P, hipStream_t s) {
+  if (P.xf)
+    return P.xf_type == kBF16 ? launch_token<kBF16>(P, s)
+           : P.xf_type == kF16 ? launch_token<kF16>(P, s)
+                               : launch_token<kF32>(P, s);
   const dim3 grid((unsigned)((((int64_t)P.M + kT - 1) / kT) * ((P.N + kT - 1) / kT)));
   if (P.w2)
     hipLaunchKernelGGL((int8_any_kernel<true>), grid, dim3(256), 0, s, P);

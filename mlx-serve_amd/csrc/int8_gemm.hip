@@ -241,15 +241,11 @@ hipError_t launch_gemm(const Int8Params& P, hipStream_t s) {
 
 }  // namespace
 
-// Rows on 16 bytes and offsets of a tile within 31 bits.
-bool int8_gemm_supported(int64_t N, int64_t K, const void* x, int64_t ldx, const void* w, const void* w2) {
-  return ((uintptr_t)x | (uintptr_t)ldx | (uintptr_t)w | (uintptr_t)w2 | (uintptr_t)K) % 16 == 0;
-}
-
 // Tile and K splits: the fewest estimated microseconds over rounds of 256 blocks (one a CU) x
-// steps, plus a split's int32 partials written and read back and the reduce launch. Depends
-// on the sizes alone (not on pointers), so the workspace can be asked for ahead.
-void int8_gemm_plan(Int8Params& P) {
+// steps, plus a split's int32 partials written and read back and the reduce launch; at least the
+// time that the operands take from HBM. Depends on the sizes alone (not on pointers), so the
+// workspace can be asked for ahead.
+double int8_gemm_plan(Int8Params& P) {
   const int steps = (P.K + kBK - 1) / kBK;
   const int banks = P.banks;
   struct Tile { int bm, bn; double us; };
@@ -270,6 +266,7 @@ void int8_gemm_plan(Int8Params& P) {
       }
     }
   }
+  return 3.5 + std::max(best, ((double)banks * P.N + P.M) * P.K / 4.4e6);
 }
 
 hipError_t launch_int8_gemm(const Int8Params& P, hipStream_t s) {

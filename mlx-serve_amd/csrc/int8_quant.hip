@@ -1,11 +1,5 @@
 // Token (row) quantization to int8, and the element-wise half of the SwiGLU gradient.
 //
-// Quantization: s = max_k |x_k| / 127 rounded once to fp32, q_k the integer nearest to x_k / s,
-// ties to even, exactly: t = x * (1/s) is within a few units of 2^-24 of the quotient, so its
-// nearest integer q is right unless the quotient lies next to a border, and r = x - q s is exact
-// in one fma (x and s have 24 bits, |r| < s, and both are multiples of s's last bit, or q = 0).
-// So |r| < s/2 proves q, and the rare others are settled from r.
-//
 // Memory-bound: a row is read once and held in registers between the maximum and the codes.
 #include "int8.h"
 
@@ -13,54 +7,6 @@ namespace mi {
 namespace {
 
 using namespace i8;
-
-constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: v + kMagic rounds v to an integer (ties to
-                                      // even), whose two's complement is the sum's low bits
-constexpr float kTiny = 0x1p-100f;    // below, x and s are scaled by 2^100 (exact)
-
-struct RowScale {
-  float s, inv, half;
-  bool fin, tiny;  // codes are 0 unless s is finite and not 0
-};
-
-MI_DEV RowScale row_scale(uint32_t maxbits) {
-  RowScale r;
-  r.s = __uint_as_float(maxbits) / 127.f;
-  r.fin = r.s > 0.f && r.s < __builtin_inff();
-  r.tiny = r.s < kTiny;
-  r.inv = r.fin ? 1.f / (r.tiny ? r.s * 0x1p100f : r.s) : 0.f;
-  r.half = 0.5f * r.s;
-  return r;
-}
-
-// any row and value
-MI_DEV int code_of(float x, const RowScale& R) {
-  if (!R.fin) return 0;
-  const float s = R.tiny ? R.s * 0x1p100f : R.s;
-  if (R.tiny) x *= 0x1p100f;
-  float q = rintf(x * R.inv);
-  const float d = fmaf(-q, s, x);
-  const float away = d > 0.f ? 1.f : -1.f, h = 0.5f * s;
-  if (fabsf(d) > h || (fabsf(d) == h && ((int)q & 1))) q += away;
-  return (int)fminf(fmaxf(q, -127.f), 127.f);
-}
-
-// four codes in a dword
-MI_DEV uint32_t codes4(const float (&x)[4], const RowScale& R) {
-  uint32_t t[4];
-  bool sure = R.fin && !R.tiny;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float v = fmaf(x[i], R.inv, kMagic);
-    t[i] = __float_as_uint(v);
-    sure = sure && fabsf(fmaf(-(v - kMagic), R.s, x[i])) < R.half;
-  }
-  if (!sure) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) t[i] = (uint32_t)code_of(x[i], R);
-  }
-  return perm_b32(perm_b32(t[3], t[2], 0x0C0C0400u), perm_b32(t[1], t[0], 0x0C0C0400u), 0x05040100u);
-}
 
 // Bits of |x| compare as the values do, and a NaN above infinity: the integer maximum keeps it.
 template <int T>

@@ -424,13 +424,23 @@ def _i8_linear(N, K, dev, *banks):
 
 def _i8_call(fn, dev, need, *args):
     """One library call on dev's current stream, with a workspace from torch's allocator: calls on
-    other streams and graphs captured from them have others."""
+    other streams and graphs captured from them have others. need None: a call without one."""
     if dev.index is not None and dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return _i8_call(fn, dev, need, *args)
-    need = max(need, 0)  # sizes out of range: the call refuses them
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    check(fn(*args, _ptr(ws), need, ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)))
+    # (the raw handle: building a Stream object costs as much as a launch)
+    stream = torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    if need is None:
+        check(fn(*args, stream))
+    elif need > 0:
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        check(fn(*args, ws.data_ptr(), need, stream))
+    else:  # none, or sizes out of range, which the call refuses
+        check(fn(*args, None, 0, stream))
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
 
 
 def int8_quantize(x):
@@ -443,10 +453,7 @@ def int8_quantize(x):
     K = x.shape[-1]
     q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
     s = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    L = lib()
-    _i8_call(lambda q, s, x, rows, K, code, ws, need, stream:
-             L.mi_int8_quantize(q, s, x, rows, K, code, stream),
-             x.device, 0, _ptr(q), _ptr(s), _ptr(x), x.numel() // K, K, code)
+    _i8_call(lib().mi_int8_quantize, x.device, None, _at(q), _at(s), _at(x), x.numel() // K, K, code)
     return q, s
 
 
@@ -480,8 +487,8 @@ def int8_matmul(x, w, w_scales, x_scales=None, bias=None, dtype=None):
     M = x.numel() // K if K else 0
     y = torch.empty(x.shape[:-1] + (N,), dtype=dtype, device=x.device)
     L = lib()
-    _i8_call(L.mi_int8_matmul, x.device, L.mi_int8_forward_workspace(M, N, K, 1, xt), _ptr(y),
-             _ptr(x), _ptr(x_scales), _ptr(w), _ptr(w_scales), _ptr(bias), M, N, K, xt, yt)
+    _i8_call(L.mi_int8_matmul, x.device, L.mi_int8_forward_workspace(M, N, K, 1, xt), _at(y),
+             _at(x), _at(x_scales), _at(w), _at(w_scales), _at(bias), M, N, K, xt, yt)
     return y
 
 
@@ -499,8 +506,8 @@ def int8_gate_up_swiglu(x, wg, sg, wu, su, x_scales=None, dtype=None, save=False
     gate = torch.empty(shape, dtype=dtype, device=x.device) if save else None
     up = torch.empty(shape, dtype=dtype, device=x.device) if save else None
     L = lib()
-    _i8_call(L.mi_int8_gate_up_swiglu, x.device, L.mi_int8_forward_workspace(M, N, K, 2, xt), _ptr(y),
-             _ptr(gate), _ptr(up), _ptr(x), _ptr(x_scales), _ptr(wg), _ptr(sg), _ptr(wu), _ptr(su),
+    _i8_call(L.mi_int8_gate_up_swiglu, x.device, L.mi_int8_forward_workspace(M, N, K, 2, xt), _at(y),
+             _at(gate), _at(up), _at(x), _at(x_scales), _at(wg), _at(sg), _at(wu), _at(su),
              M, N, K, xt, yt)
     return (y, gate, up) if save else y
 
@@ -518,7 +525,7 @@ def int8_matmul_backward(dy, w, w_scales):
     dx = torch.empty(dy.shape[:-1] + (K,), dtype=dy.dtype, device=dy.device)
     L = lib()
     _i8_call(L.mi_int8_matmul_backward, dy.device, L.mi_int8_backward_workspace(M, N, K, 1, code),
-             _ptr(dx), _ptr(dy), _ptr(w), _ptr(w_scales), M, N, K, code)
+             _at(dx), _at(dy), _at(w), _at(w_scales), M, N, K, code)
     return dx
 
 
@@ -538,8 +545,8 @@ def int8_gate_up_swiglu_backward(dy, gate, up, wg, sg, wu, su):
     dgate, dup = torch.empty_like(dy), torch.empty_like(dy)
     L = lib()
     _i8_call(L.mi_int8_gate_up_swiglu_backward, dy.device,
-             L.mi_int8_backward_workspace(M, N, K, 2, code), _ptr(dx), _ptr(dgate), _ptr(dup),
-             _ptr(dy), _ptr(gate), _ptr(up), _ptr(wg), _ptr(sg), _ptr(wu), _ptr(su), M, N, K, code)
+             L.mi_int8_backward_workspace(M, N, K, 2, code), _at(dx), _at(dgate), _at(dup),
+             _at(dy), _at(gate), _at(up), _at(wg), _at(sg), _at(wu), _at(su), M, N, K, code)
     return dx, dgate, dup
 
 
