@@ -45,7 +45,9 @@ MI_DEV u32x2_t codes_f16(uint32_t w) {
   return u32x2_t{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
 }
 
-MI_DEV i32x2_t read_tr8(const unsigned char* p) {
+// (__restrict__ gives the read an alias scope: without one the compiler takes every LDS DMA in flight
+// for a write to it and waits for all of them, vmcnt(0), each step.)
+MI_DEV i32x2_t read_tr8(const unsigned char* __restrict__ p) {
   return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2_t*)p);
 }
 
@@ -103,16 +105,15 @@ int8_bwd_kernel(Int8BwdParams P) {
   auto wbase = [&](const Cursor& c) { return P.w[c.seg >= P.terms] + (size_t)c.n * K; };
   // stages past the range load through resources of zero records (zeros, no traffic), rows from N
   // on and columns from K on out of bounds
-  auto issue = [&](const Cursor& c, int slot) __attribute__((always_inline)) {
+  auto issue = [&](const Cursor& c, int slot, int j) __attribute__((always_inline)) {  // instruction j
     const bool on = c.st < ns;
-    const int rows = min(kBN_, N - c.n);
     unsigned char* b = smem + slot * kStage;
-#pragma unroll
-    for (int i = 0; i < XI; ++i)
-      dma16(rsrc(abase(c), on ? abytes : 0), b + (wave * XI + i) * 1024, xo[i], c.n * 2);
-#pragma unroll
-    for (int i = 0; i < WI; ++i)
+    if (j < XI) {
+      dma16(rsrc(abase(c), on ? abytes : 0), b + (wave * XI + j) * 1024, xo[j], c.n * 2);
+    } else {
+      const int i = j - XI, rows = min(kBN_, N - c.n);
       dma16(rsrc(wbase(c), on ? rows * K : 0), b + kW + (wave * WI + i) * 1024, wr[i] < rows ? wo[i] : kOOB, 0);
+    }
   };
   // L2 prefetch: waves 0-3 the rows of a, 64 a wave; waves 4, 5 the two lines of the rows of w
   const int h = min(4, mtiles - at.mt / 4 * 4);
@@ -135,7 +136,7 @@ int8_bwd_kernel(Int8BwdParams P) {
   for (int a = 0; a < NT; ++a)
 #pragma unroll
     for (int i = 0; i < MT; ++i) acc[a][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  u32x4_t X[2][MT];
+  u32x4_t X[2][MT], Wf[2];  // Wf: the codes of one tile as fp16, and the next one's
   i32x2_t A[2][NT];
   // half e: values n = 16 q + 8 e .. + 7 of both operands (slot 2q + e of a row of a)
   const int fo0 = fr * 128 + (((2 * q) ^ xswz(fr)) << 4), fo1 = fr * 128 + (((2 * q + 1) ^ xswz(fr)) << 4);
@@ -144,28 +145,52 @@ int8_bwd_kernel(Int8BwdParams P) {
   int ao[NT];
 #pragma unroll
   for (int a = 0; a < NT; ++a) ao[a] = kW + nr * BN + (((wn * NT + a) ^ nswz<BN>(nr)) << 4) + 8 * (fr & 1);
-  auto frags = [&](int slot, int e) __attribute__((always_inline)) {
-    const unsigned char* b = smem + slot * kStage;
+  auto read_a = [&](int slot, int e) __attribute__((always_inline)) {
 #pragma unroll
-    for (int a = 0; a < NT; ++a) A[e][a] = read_tr8(b + ao[a] + e * 8 * BN);
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-      X[e][i] = *reinterpret_cast<const u32x4_t*>(b + xr + (e ? fo1 : fo0) + 16 * i * 128);
+    for (int a = 0; a < NT; ++a) A[e][a] = read_tr8(smem + slot * kStage + ao[a] + e * 8 * BN);
   };
-  auto products = [&](int e) __attribute__((always_inline)) {
+  auto read_x = [&](int slot, int e, int i) __attribute__((always_inline)) {
+    X[e][i] = *reinterpret_cast<const u32x4_t*>(smem + slot * kStage + xr + (e ? fo1 : fo0) + 16 * i * 128);
+  };
+  auto to_f16 = [&](int e, int a) -> u32x4_t {
+    const u32x2_t lo = codes_f16((uint32_t)A[e][a].x), hi = codes_f16((uint32_t)A[e][a].y);
+    return u32x4_t{lo.x, lo.y, hi.x, hi.y};
+  };
+  // The products of half e, one tile of codes at a time. Beside a tile's MFMAs: the next tile's
+  // codes to fp16, and a part of the next half's fragment reads (its codes first: the last tile's
+  // neighbour is their first) from stage `rs`, and of the DMA where `dma`.
+  auto half = [&](int e, int rs, bool dma, const Cursor& c, int slot) __attribute__((always_inline)) {
+    constexpr int kX = NT > 1 ? (MT + NT - 2) / (NT - 1) : MT;  // x reads of the tiles after the first
 #pragma unroll
     for (int a = 0; a < NT; ++a) {
-      const u32x2_t lo = codes_f16((uint32_t)A[e][a].x), hi = codes_f16((uint32_t)A[e][a].y);
-      const u32x4_t w = {lo.x, lo.y, hi.x, hi.y};
+      if (a == 0) read_a(rs, e ^ 1);
 #pragma unroll
-      for (int i = 0; i < MT; ++i) acc[a][i] = mfma_f16(w, X[e][i], acc[a][i]);
+      for (int i = 0; i < kX; ++i)
+        if (a > 0 && (a - 1) * kX + i < MT) read_x(rs, e ^ 1, (a - 1) * kX + i);
+      if (dma) {
+#pragma unroll
+        for (int j = a; j < XI + WI; j += NT) issue(c, slot, j);
+      }
+      Wf[(a + 1) & 1] = a + 1 < NT ? to_f16(e, a + 1) : to_f16(e ^ 1, 0);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) acc[a][i] = mfma_f16(Wf[a & 1], X[e][i], acc[a][i]);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+        if (i % 4 == 1) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
+  static_assert(NT % 2 == 0, "a half ends on the tile buffer it began on");
 
   Cursor ci = start(0), cp = start(R);
 #pragma unroll
   for (int s = 0; s < R; ++s) {
-    issue(ci, s);
+#pragma unroll
+    for (int j = 0; j < XI + WI; ++j) issue(ci, s, j);
     prefetch(cp);
     step(ci);
     step(cp);
@@ -174,38 +199,23 @@ int8_bwd_kernel(Int8BwdParams P) {
   wait_vm(1 + (R - 1) * (XI + WI + 1));
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_sched_barrier(0);
-  frags(0, 0);
+  read_a(0, 0);
+#pragma unroll
+  for (int i = 0; i < MT; ++i) read_x(0, 0, i);
+  Wf[0] = to_f16(0, 0);
   int slot = 0;
 #pragma unroll 1
   for (int t = 0; t < ns; ++t) {
     const int next = slot + 1 == R ? 0 : slot + 1;
-    frags(slot, 1);
-    products(0);
-#pragma unroll
-    for (int r = 0; r < MT * NT; ++r) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      if (r < MT + NT) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
-    }
-    __builtin_amdgcn_sched_barrier(0);
+    half(0, slot, false, ci, slot);
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): this wave's reads of stage t
     wait_vm(1 + (R - 2) * (XI + WI + 1));
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
-    frags(next, 0);
-    issue(ci, slot);
+    half(1, next, true, ci, slot);
     prefetch(cp);
     step(ci);
     step(cp);
-    products(1);
-#pragma unroll
-    for (int r = 0; r < MT * NT; ++r) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      if (r < MT + NT) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
-      if (r % 2 == 0) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
-    }
-    __builtin_amdgcn_sched_barrier(0);
     slot = next;
   }
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // no DMA may outlive the block

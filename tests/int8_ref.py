@@ -48,8 +48,8 @@ def matmul(q, sx, w, sw, bias=None):
 
 def gate_up(q, sx, wg, sg, wu, su):
     """(y, gate, up, tolerance of y, of gate, of up). silu's relative condition number is at most
-    1 + |g|: 3 roundings of g count that much, the exponential is within 2 of its own U (one ulp), and
-    1 + e, the quotient and the products round once each. e^-g overflows below g = -88: 2^-120."""
+    1 + |g|: 3 roundings of g count that much; the exponential is off by 2 + 1.25 |g| (as in grads), and
+    1 + e, the reciprocal (2) and the products add 8 at most. e^-g overflows below g = -88: 2^-120."""
     g, u = product(q, sx, wg, sg), product(q, sx, wu, su)
     y = g * torch.special.expit(g) * u
     rel = U * (3 * (1 + g.abs()) + 2 * (1 + g.abs()) + 3 + 5)
@@ -61,16 +61,21 @@ def gate_up(q, sx, wg, sg, wu, su):
 
 
 def grads(dy, g, u):
-    """(dgate, dup, tolerances before their rounding): s within 5 U of its value (exponential 2, sum,
-    quotient; its exponent's rounding |g| more); 1 - s has that as an absolute error."""
+    """(dgate, dup, tolerances before their rounding). s = 1 / (1 + 2^t), t = g log2(e): one ulp, 2 U, for
+    the exponential and as much for the reciprocal, U for the sum; t is off by its rounding, U |t|,
+    and by the constant's (0.23 U relative), which 2^t turns into 1.23 U |g|. 1 - s has the error of s
+    as an absolute error."""
     dy, g, u = dy.double(), g.double(), u.double()
     s = torch.special.expit(g)
     dg, du = dy * u * (s + g * s * (1 - s)), dy * g * s
-    es = U * (5 + g.abs())
+    es = U * (5 + 1.25 * g.abs())
     tg = (dy * u * s).abs() * ((1 + g.abs() * (1 - s)) * (es + 4 * U) + g.abs() * (s * es + 3 * U))
     tu = du.abs() * (es + 2 * U)
-    tiny = 2.0 ** -120
-    return dg, du, 1.01 * tg + (dy * u).abs() * tiny, 1.01 * tu + (dy * g).abs() * tiny
+    # the reciprocal gives 0 for an s below 2^-126 (no subnormals): an absolute error of 2^-126 that
+    # dgate multiplies by 1 + g (1 - s), at most 1 + |g|, and dup by g; twice that for the products
+    # on the way, which may be subnormal too
+    tiny = 2.0 ** -125
+    return dg, du, 1.01 * tg + (dy * u).abs() * (1 + g.abs()) * tiny, 1.01 * tu + (dy * g).abs() * tiny
 
 
 def through(a, ta, w, sw, t, top):
