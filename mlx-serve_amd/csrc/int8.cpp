@@ -68,7 +68,7 @@ int64_t forward_need(mi::Int8Params& P, int64_t M, int64_t N, int64_t K, int x_d
   P.K = (int)K;
   P.ks = 1;
   P.nt = 0;
-  if (K % 16 == 0) {  // up to 16 rows the few-row kernel, up to 64 the one that should be faster
+  if (K % 16 == 0) {  // up to 16 rows the few-row kernel, up to 128 the one that should be faster
     const double few = M <= mi::kInt8FewRows ? mi::int8_gemv_plan(P) : 0.0;
     const int nt = P.nt;
     const double tiles = M > 16 ? mi::int8_gemm_plan(P) : 0.0;

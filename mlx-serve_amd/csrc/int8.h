@@ -11,7 +11,7 @@ enum FloatType { kBF16 = 0, kF16 = 1, kF32 = 2 };
 
 // The int32 sum of K products of codes is exact up to here: 131071 * 128 * 128 < 2^31.
 constexpr int64_t kInt8MaxK = 131071;
-constexpr int64_t kInt8FewRows = 64;  // rows that int8_gemv.hip can take
+constexpr int64_t kInt8FewRows = 128;  // rows that int8_gemv.hip can take
 
 // y[m,n] = sx[m] * sw[n] * sum_k x[m,k] w[n,k] (+ bias[n]), or with a second bank (w2)
 // y = silu(g) * u of the two products, which go to `gate` and `up` as well where given.
@@ -32,9 +32,9 @@ struct Int8Params {
   int M, N, K;
   int type;   // FloatType of y, bias, gate and up
   int banks;  // 1, or 2 with w2
-  // int8_gemm.hip: rows of a tile; K ranges over blocks and 128-code steps of one, ks > 1
+  // int8_gemm.hip: rows of x and of w (both banks) of a tile; K ranges over blocks and 128-code steps of one, ks > 1
   // through int32 sums [ks][banks][M][N] in `part`
-  int bm, ks, sps;
+  int bm, bn, ks, sps;
   int32_t* part;
   int nt;    // int8_gemv.hip: 16-row tiles of a wave; 0: another kernel
   bool vec;  // y, gate, up, part rows of four columns on one store (N and pointers)
@@ -52,7 +52,7 @@ struct Int8BwdParams {
   int banks, terms, np;
   int M, N, K;
   int type;
-  int bm, ks, sps;  // int8_bwd.hip: rows of a tile, ranges of sps 64-value steps over the parts
+  int bm, bn, ks, sps;  // int8_bwd.hip: rows and columns of a tile, ranges of sps 64-value steps over the parts
   bool vec;
 };
 
@@ -83,7 +83,7 @@ hipError_t launch_int8_gemm(const Int8Params& P, hipStream_t s);
 hipError_t launch_int8_any(const Int8Params& P, hipStream_t s);
 hipError_t launch_int8_grad(const Int8GradParams& P, hipStream_t s);
 bool int8_bwd_supported(int64_t K, const void* w, const void* w2);
-void int8_bwd_plan(Int8BwdParams& P);  // from M, K, np, banks and terms: bm, ks, sps
+void int8_bwd_plan(Int8BwdParams& P);  // from M, K, np, banks and terms: bm, bn, ks, sps
 hipError_t launch_int8_bwd(const Int8BwdParams& P, hipStream_t s);
 hipError_t launch_int8_bwd_any(const Int8BwdParams& P, hipStream_t s);
 

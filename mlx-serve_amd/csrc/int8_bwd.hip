@@ -51,8 +51,12 @@ MI_DEV i32x2_t read_tr8(const unsigned char* __restrict__ p) {
   return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2_t*)p);
 }
 
+// waves a SIMD: 2 (one block a CU), 4 for the small tiles (two blocks)
+constexpr int eu_waves(int bm, int bn) { return bm * bn <= 128 * 128 ? 4 : 2; }
+
 template <int BM, int BN, int R, bool SPLIT>
-__global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
+__global__ void __launch_bounds__(512)
+    __attribute__((amdgpu_waves_per_eu(eu_waves(BM, BN), eu_waves(BM, BN))))
 int8_bwd_kernel(Int8BwdParams P) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   constexpr int MT = BM / 32, NT = BN / 64;   // 16-row / 16-column tiles of a wave
@@ -282,21 +286,25 @@ bool int8_bwd_supported(int64_t K, const void* w, const void* w2) {
   return ((uintptr_t)w | (uintptr_t)w2 | (uintptr_t)K) % 16 == 0;
 }
 
-// As int8_gemm_plan.
+// As int8_gemm_plan. Measured, us with the gradient's own pass, 256x256 / 128x256 / 128x128 / 64x128 tiles:
+//   dx [M,4096], sum of 4096   128 rows 31 / 31 / 26 / 25   512 44 / 39 / 41 / 46    2048  87 /  81 /  91 / 126
+//   dx [M,14336], sum of 4096  128 rows 46 / 41 / 43 / 47   512 80 / 75 / 84 / 124   2048 219 / 285 / 280 / 410
+//   dx [M,4096], gate + up sums of 14336  77 rows 69 / 61 / 59 / 74    4096 847 / 1078 / 1197 / 1690
 void int8_bwd_plan(Int8BwdParams& P) {
   const int steps = P.banks * P.terms * (P.np / kBN_);
-  struct Tile { int bm, bn; double us; };
-  constexpr Tile kTiles[] = {{256, 256, 1.7}, {128, 256, 1.0}, {64, 128, 0.5}};
+  constexpr TileCost kTiles[] = {
+      {256, 256, 1.55, 0.0, 8.0}, {128, 256, 1.0, 0.0, 4.0}, {128, 128, 0.75, 1.0, 3.0}, {64, 128, 0.6, 0.84, 3.0}};
   double best = 1e30;
-  for (const Tile& t : kTiles) {
+  for (const TileCost& t : kTiles) {
     const int64_t tiles = (int64_t)((P.M + t.bm - 1) / t.bm) * ((P.K + t.bn - 1) / t.bn);
     for (int k = 1; k <= std::max(1, steps / 4) && k <= 64; ++k) {
       const int sps = (steps + k - 1) / k, ks = (steps + sps - 1) / sps;
-      const double part = ks > 1 ? (double)ks * P.M * P.K * 8 / 5e6 + 4.0 : 0.0;
-      const double cost = (double)((tiles * ks + 255) / 256) * (sps * t.us + 2.0) + part;
+      const double part = ks > 1 ? (double)ks * P.M * P.K * 8 / 5e6 + 3.0 : 0.0;
+      const double cost = tile_us(t, tiles * ks, sps) + part;
       if (cost < best - 1e-9) {
         best = cost;
         P.bm = t.bm;
+        P.bn = t.bn;
         P.ks = ks;
         P.sps = sps;
       }
@@ -306,8 +314,9 @@ void int8_bwd_plan(Int8BwdParams& P) {
 
 hipError_t launch_int8_bwd(const Int8BwdParams& P, hipStream_t s) {
   const hipError_t e = P.bm == 256   ? launch_tile<256, 256, 3>(P, s)
-                       : P.bm == 128 ? launch_tile<128, 256, 4>(P, s)
-                                     : launch_tile<64, 128, 6>(P, s);
+                       : P.bm == 128 ? (P.bn == 256 ? launch_tile<128, 256, 4>(P, s)
+                                                    : launch_tile<128, 128, 3>(P, s))
+                                     : launch_tile<64, 128, 4>(P, s);
   if (e != hipSuccess || P.ks == 1) return e;
   int64_t g = ((int64_t)P.M * P.K / 4 + 255) / 256;
   if (g > 8192) g = 8192;

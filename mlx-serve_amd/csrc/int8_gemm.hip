@@ -37,8 +37,12 @@ constexpr int kBK = 128;
 template <int BM, int BN, int R>
 constexpr int lds_bytes() { return R * (BM + BN) * kBK + 2048; }
 
+// waves a SIMD: 2 (one block a CU), 4 for the small tiles (two blocks, whose starts and ends overlap)
+constexpr int eu_waves(int bm, int bn) { return bm * bn <= 128 * 128 ? 4 : 2; }
+
 template <bool DUAL, int BM, int BN, int R, bool SPLIT>
-__global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
+__global__ void __launch_bounds__(512)
+    __attribute__((amdgpu_waves_per_eu(eu_waves(BM, BN), eu_waves(BM, BN))))
 int8_gemm_kernel(Int8Params P) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   constexpr int MT = BM / 32, NT = BN / 64;    // 16-row tiles of a wave
@@ -230,8 +234,9 @@ hipError_t launch_tile(const Int8Params& P, hipStream_t s) {
 template <bool DUAL>
 hipError_t launch_gemm(const Int8Params& P, hipStream_t s) {
   hipError_t e = P.bm == 256   ? launch_tile<DUAL, 256, 256, 2>(P, s)
-                 : P.bm == 128 ? launch_tile<DUAL, 128, 256, 3>(P, s)
-                               : launch_tile<DUAL, 64, 128, 4>(P, s);
+                 : P.bm == 128 ? (P.bn == 256 ? launch_tile<DUAL, 128, 256, 3>(P, s)
+                                              : launch_tile<DUAL, 128, 128, 2>(P, s))
+                               : launch_tile<DUAL, 64, 128, 3>(P, s);
   if (e != hipSuccess || P.ks == 1) return e;
   int64_t g = ((int64_t)P.M * ((P.N + 3) / 4) + 255) / 256;
   if (g > 8192) g = 8192;
@@ -241,32 +246,36 @@ hipError_t launch_gemm(const Int8Params& P, hipStream_t s) {
 
 }  // namespace
 
-// Tile and K splits: the fewest estimated microseconds over rounds of 256 blocks (one a CU) x
-// steps, plus a split's int32 partials written and read back and the reduce launch; at least the
-// time that the operands take from HBM. Depends on the sizes alone (not on pointers), so the
-// workspace can be asked for ahead.
+// Tile and K splits: the fewest estimated microseconds, from the blocks' steps, a split's int32
+// partials written and read back with the reduce launch, and the time that the operands take
+// from HBM at least. Depends on the sizes alone (not on pointers), so the workspace can be asked
+// for ahead. Measured, us, with 256x256 / 128x256 / 128x128 / 64x128 tiles:
+//   [14336,4096]  128 rows 35 / 33 / 29 / 27   512 57 / 41 / 47 / 61   2048 128 / 154 / 153 / 199
+//   [4096,4096]   128 rows 25 / 24 / 20 / 17   512 34 / 28 / 26 / 21   2048  55 /  40 /  45 /  61
+//   [4096,14336]  128 rows 34 / 31 / 28 / 29   512 54 / 48 / 57 / 63   2048 124 / 117 / 140 / 193
+//   gate + up [14336,4096] 256 rows 61 / 43 / 50 / 62, 1024 120 / 141 / 153 / 194
 double int8_gemm_plan(Int8Params& P) {
-  const int steps = (P.K + kBK - 1) / kBK;
-  const int banks = P.banks;
-  struct Tile { int bm, bn; double us; };
-  constexpr Tile kTiles[] = {{256, 256, 1.8}, {128, 256, 1.1}, {64, 128, 0.55}};
+  const int steps = (P.K + kBK - 1) / kBK, banks = P.banks;
+  constexpr TileCost kTiles[] = {
+      {256, 256, 1.72, 0.0, 8.0}, {128, 256, 1.03, 0.0, 4.0}, {128, 128, 0.75, 1.13, 3.0}, {64, 128, 0.55, 0.8, 3.0}};
   double best = 1e30;
-  for (const Tile& t : kTiles) {
+  for (const TileCost& t : kTiles) {
     const int on = t.bn / banks;
     const int64_t tiles = (int64_t)((P.M + t.bm - 1) / t.bm) * ((P.N + on - 1) / on);
     for (int k = 1; k <= std::max(1, steps / 4) && k <= 64; ++k) {
       const int sps = (steps + k - 1) / k, ks = (steps + sps - 1) / sps;
-      const double part = ks > 1 ? (double)ks * banks * P.M * P.N * 8 / 5e6 + 4.0 : 0.0;
-      const double cost = (double)((tiles * ks + 255) / 256) * (sps * t.us + 2.0) + part;
+      const double part = ks > 1 ? (double)ks * banks * P.M * P.N * 8 / 5e6 + 3.0 : 0.0;
+      const double cost = tile_us(t, tiles * ks, sps) + part;
       if (cost < best - 1e-9) {
         best = cost;
         P.bm = t.bm;
+        P.bn = t.bn;
         P.ks = ks;
         P.sps = sps;
       }
     }
   }
-  return 3.5 + std::max(best, ((double)banks * P.N + P.M) * P.K / 4.4e6);
+  return 3.0 + std::max(best, ((double)banks * P.N + P.M) * P.K / 4.4e6);
 }
 
 hipError_t launch_int8_gemm(const Int8Params& P, hipStream_t s) {

@@ -1,4 +1,4 @@
-// Int8 products of few rows (up to 64): decode. The weights are read once, so their bytes bound it.
+// Int8 products of few rows (up to 128): decode, and short prompts through small matrices. The weights are read once, so their bytes bound it.
 //
 // Block: WK waves that share 16 NT rows of w (of both banks, with two) and split K between them;
 // a wave streams its part of those rows straight into registers (one instruction reads 16 rows x 64
@@ -74,7 +74,7 @@ MI_DEV float quantize_token(const u32x4_t (&v)[XV], int K, unsigned char* xs, ui
 }
 
 template <bool DUAL, int MT, int NT, int WK, int U, int XV>
-__global__ void __launch_bounds__(WK * 64, MT == 1 ? 8 : 4) int8_gemv_kernel(Int8Params P) {
+__global__ void __launch_bounds__(WK * 64, MT == 1 ? 8 : MT <= 4 ? 4 : 2) int8_gemv_kernel(Int8Params P) {
   constexpr int B = DUAL ? 2 : 1;
   constexpr bool FUSE = XV > 0;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -193,7 +193,12 @@ hipError_t launch_tiles(const Int8Params& P, hipStream_t s) {
   if (P.M <= 16) return launch<DUAL, 1, NT, 8, DUAL || NT == 2 ? 2 : 4, 0>(P, s);
   if (P.M <= 32) return launch<DUAL, 2, NT, 8, 2, 0>(P, s);
   if (P.M <= 48) return launch<DUAL, 3, NT, 8, 2, 0>(P, s);
-  return launch<DUAL, 4, NT, 8, 2, 0>(P, s);
+  if (P.M <= 64) return launch<DUAL, 4, NT, 8, 2, 0>(P, s);
+  if constexpr (NT == 1) {
+    if (P.M <= 96) return launch<DUAL, 6, 1, 8, 2, 0>(P, s);
+    return launch<DUAL, 8, 1, 8, 2, 0>(P, s);
+  }
+  return hipErrorInvalidValue;  // (the plan takes one tile above 64 rows)
 }
 
 template <bool DUAL>
@@ -216,7 +221,7 @@ hipError_t launch_rows(const Int8Params& P, hipStream_t s) {
 // they leave a block for each CU. Measured, one / two tiles a wave: [14336,4096] 2 rows 14.7 /
 // 16.0 us, 16 rows 20.9 / 17.5; [4096,14336] 16 rows 20.1 / 23.7.
 double int8_gemv_plan(Int8Params& P) {
-  P.nt = P.banks == 1 && P.M > 8 && P.N >= 32 * 256 ? 2 : 1;
+  P.nt = P.banks == 1 && P.M > 8 && P.M <= 64 && P.N >= 32 * 256 ? 2 : 1;
   const double blocks = (double)((P.N + 16 * P.nt - 1) / (16 * P.nt));
   return 3.0 + std::max(1.0, blocks / 256) * (16.0 * P.nt * P.banks + P.M) * P.K / 25e3;
 }

@@ -39,5 +39,19 @@ MI_DEV void wait_vm(int n) {
 }
 
 
+// A tile of the matrix kernels for their plans: microseconds a step of a block that has its CU to
+// itself, of two that share it (0: a block fills the CU), and beside the steps (start, end).
+struct TileCost {
+  int bm, bn;
+  double alone, paired, ends;
+};
+// `tiles` blocks of `steps` steps on 256 CUs
+inline double tile_us(const TileCost& t, int64_t tiles, int steps) {
+  const int64_t per_cu = (tiles + 255) / 256;
+  const double one = steps * t.alone + t.ends;
+  if (t.paired == 0.0) return (double)per_cu * one;
+  return (double)(per_cu / 2) * (steps * t.paired + t.ends) + (per_cu % 2 ? one : 0.0);
+}
+
 }  // namespace i8
 }  // namespace mi

@@ -402,22 +402,23 @@ def gather_qmv_down_reduce(act, wd, sd, bd, inds, scores, group_size=None, bits=
 
 
 # ------------------------------------------- int8 weights and activations --
+# One decoded token costs a few microseconds on the GPU, so these wrappers read each attribute once.
 _I8 = {torch.bfloat16: DT_BFLOAT16, torch.float16: DT_FLOAT16, torch.float32: DT_FLOAT32}
 
 
 def _i8_type(dtype, what):
-    if dtype not in _I8:
+    code = _I8.get(dtype)
+    if code is None:
         raise MiError(MI_ERR_INVALID, f"{what} dtype {dtype} not supported (bfloat16, float16, float32)")
-    return _I8[dtype]
+    return code
 
 
 def _i8_linear(N, K, dev, *banks):
     """Every bank is int8 [N, K] with fp32 scales [N], on the device of the activations."""
     for w, s in banks:
         _contig(w, s)
-        _require(w.dtype == torch.int8 and w.dim() == 2, "weights must be int8 [N, K]")
-        _require(w.shape[0] == N and w.shape[1] == K,
-                 f"weights {tuple(w.shape)} do not match [{N}, {K}]")
+        _require(w.dtype == torch.int8, "weights must be int8 [N, K]")
+        _require(tuple(w.shape) == (N, K), f"weights {tuple(w.shape)} do not match [{N}, {K}]")
         _require(s.dtype == torch.float32 and s.numel() == N, "channel scales must be float32 [N]")
         _require(w.device == dev and s.device == dev, "tensors on different devices")
 
@@ -425,18 +426,21 @@ def _i8_linear(N, K, dev, *banks):
 def _i8_call(fn, dev, need, *args):
     """One library call on dev's current stream, with a workspace from torch's allocator: calls on
     other streams and graphs captured from them have others. need None: a call without one."""
-    if dev.index is not None and dev.index != torch.cuda.current_device():
+    at = dev.index
+    if at != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return _i8_call(fn, dev, need, *args)
     # (the raw handle: building a Stream object costs as much as a launch)
-    stream = torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    stream = torch._C._cuda_getCurrentRawStream(at)
     if need is None:
-        check(fn(*args, stream))
+        rc = fn(*args, stream)
     elif need > 0:
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        check(fn(*args, ws.data_ptr(), need, stream))
+        rc = fn(*args, ws.data_ptr(), need, stream)
     else:  # none, or sizes out of range, which the call refuses
-        check(fn(*args, None, 0, stream))
+        rc = fn(*args, None, 0, stream)
+    if rc:
+        check(rc)
 
 
 def _at(t):
@@ -448,12 +452,14 @@ def int8_quantize(x):
     [...]): scale = max |x| / 127, code = the nearest integer to x / scale, ties to even.
     For the tokens of an activation and for the output channels of a weight [N, K]."""
     _contig(x)
-    _require(x.dim() >= 1 and x.shape[-1] > 0, "x must be [..., K] with K > 0")
+    shape, dev = x.shape, x.device
+    _require(len(shape) >= 1 and shape[-1] > 0, "x must be [..., K] with K > 0")
     code = _i8_type(x.dtype, "x")
-    K = x.shape[-1]
-    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    s = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    _i8_call(lib().mi_int8_quantize, x.device, None, _at(q), _at(s), _at(x), x.numel() // K, K, code)
+    K = shape[-1]
+    q = torch.empty(shape, dtype=torch.int8, device=dev)
+    s = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
+    _i8_call(lib().mi_int8_quantize, dev, None, q.data_ptr(), s.data_ptr(), x.data_ptr(), x.numel() // K, K,
+             code)
     return q, s
 
 
@@ -461,14 +467,15 @@ def _i8_activations(x, x_scales, dtype, K):
     """(x's code, y's dtype) of a forward call."""
     _contig(x, x_scales)
     _require(x.dim() >= 1 and x.shape[-1] == K, f"x {tuple(x.shape)} must end in K={K}")
-    if x.dtype == torch.int8:
+    xd = x.dtype
+    if xd == torch.int8:
         _require(x_scales is not None, "int8 x needs x_scales")
         _require(x_scales.dtype == torch.float32 and x_scales.numel() * K == x.numel(),
                  "x_scales must be float32, one a row of x")
         _require(x_scales.device == x.device, "tensors on different devices")
         return DT_INT8, torch.bfloat16 if dtype is None else dtype
     _require(x_scales is None, "x_scales belong to int8 x")
-    return _i8_type(x.dtype, "x"), x.dtype if dtype is None else dtype
+    return _i8_type(xd, "x"), xd if dtype is None else dtype
 
 
 def int8_matmul(x, w, w_scales, x_scales=None, bias=None, dtype=None):
@@ -477,18 +484,19 @@ def int8_matmul(x, w, w_scales, x_scales=None, bias=None, dtype=None):
     x_scales. y has `dtype` (default: x's, bfloat16 for codes); bias [N] in it, or None."""
     _require(w.dim() == 2, "weights must be int8 [N, K]")
     N, K = w.shape
+    dev = x.device
     xt, dtype = _i8_activations(x, x_scales, dtype, K)
-    _i8_linear(N, K, x.device, (w, w_scales))
+    _i8_linear(N, K, dev, (w, w_scales))
     yt = _i8_type(dtype, "y")
     if bias is not None:
         _contig(bias)
-        _require(bias.dtype == dtype and bias.numel() == N and bias.device == x.device,
+        _require(bias.dtype == dtype and bias.numel() == N and bias.device == dev,
                  "bias must be [N] in y's dtype, on x's device")
     M = x.numel() // K if K else 0
-    y = torch.empty(x.shape[:-1] + (N,), dtype=dtype, device=x.device)
+    y = torch.empty(x.shape[:-1] + (N,), dtype=dtype, device=dev)
     L = lib()
-    _i8_call(L.mi_int8_matmul, x.device, L.mi_int8_forward_workspace(M, N, K, 1, xt), _at(y),
-             _at(x), _at(x_scales), _at(w), _at(w_scales), _at(bias), M, N, K, xt, yt)
+    _i8_call(L.mi_int8_matmul, dev, L.mi_int8_forward_workspace(M, N, K, 1, xt), y.data_ptr(), x.data_ptr(),
+             _at(x_scales), w.data_ptr(), w_scales.data_ptr(), _at(bias), M, N, K, xt, yt)
     return y
 
 
@@ -497,17 +505,18 @@ def int8_gate_up_swiglu(x, wg, sg, wu, su, x_scales=None, dtype=None, save=False
     (y, gate, up), the two projections for int8_gate_up_swiglu_backward."""
     _require(wg.dim() == 2, "weights must be int8 [N, K]")
     N, K = wg.shape
+    dev = x.device
     xt, dtype = _i8_activations(x, x_scales, dtype, K)
-    _i8_linear(N, K, x.device, (wg, sg), (wu, su))
+    _i8_linear(N, K, dev, (wg, sg), (wu, su))
     yt = _i8_type(dtype, "y")
     M = x.numel() // K if K else 0
     shape = x.shape[:-1] + (N,)
-    y = torch.empty(shape, dtype=dtype, device=x.device)
-    gate = torch.empty(shape, dtype=dtype, device=x.device) if save else None
-    up = torch.empty(shape, dtype=dtype, device=x.device) if save else None
+    y = torch.empty(shape, dtype=dtype, device=dev)
+    gate = torch.empty(shape, dtype=dtype, device=dev) if save else None
+    up = torch.empty(shape, dtype=dtype, device=dev) if save else None
     L = lib()
-    _i8_call(L.mi_int8_gate_up_swiglu, x.device, L.mi_int8_forward_workspace(M, N, K, 2, xt), _at(y),
-             _at(gate), _at(up), _at(x), _at(x_scales), _at(wg), _at(sg), _at(wu), _at(su),
+    _i8_call(L.mi_int8_gate_up_swiglu, dev, L.mi_int8_forward_workspace(M, N, K, 2, xt), y.data_ptr(), _at(gate),
+             _at(up), x.data_ptr(), _at(x_scales), wg.data_ptr(), sg.data_ptr(), wu.data_ptr(), su.data_ptr(),
              M, N, K, xt, yt)
     return (y, gate, up) if save else y
 
@@ -518,14 +527,15 @@ def int8_matmul_backward(dy, w, w_scales):
     _contig(dy)
     _require(w.dim() == 2, "weights must be int8 [N, K]")
     N, K = w.shape
+    dev = dy.device
     _require(dy.dim() >= 1 and dy.shape[-1] == N, f"dy {tuple(dy.shape)} must end in N={N}")
-    _i8_linear(N, K, dy.device, (w, w_scales))
+    _i8_linear(N, K, dev, (w, w_scales))
     code = _i8_type(dy.dtype, "dy")
     M = dy.numel() // N if N else 0
-    dx = torch.empty(dy.shape[:-1] + (K,), dtype=dy.dtype, device=dy.device)
+    dx = torch.empty(dy.shape[:-1] + (K,), dtype=dy.dtype, device=dev)
     L = lib()
-    _i8_call(L.mi_int8_matmul_backward, dy.device, L.mi_int8_backward_workspace(M, N, K, 1, code),
-             _at(dx), _at(dy), _at(w), _at(w_scales), M, N, K, code)
+    _i8_call(L.mi_int8_matmul_backward, dev, L.mi_int8_backward_workspace(M, N, K, 1, code), dx.data_ptr(),
+             dy.data_ptr(), w.data_ptr(), w_scales.data_ptr(), M, N, K, code)
     return dx
 
 
@@ -534,19 +544,20 @@ def int8_gate_up_swiglu_backward(dy, gate, up, wg, sg, wu, su):
     _contig(dy, gate, up)
     _require(wg.dim() == 2, "weights must be int8 [N, K]")
     N, K = wg.shape
+    dev = dy.device
     _require(dy.dim() >= 1 and dy.shape[-1] == N, f"dy {tuple(dy.shape)} must end in N={N}")
     for t, what in ((gate, "gate"), (up, "up")):
-        _require(t.shape == dy.shape and t.dtype == dy.dtype and t.device == dy.device,
+        _require(t.shape == dy.shape and t.dtype == dy.dtype and t.device == dev,
                  f"{what} must match dy in shape, dtype and device")
-    _i8_linear(N, K, dy.device, (wg, sg), (wu, su))
+    _i8_linear(N, K, dev, (wg, sg), (wu, su))
     code = _i8_type(dy.dtype, "dy")
     M = dy.numel() // N if N else 0
-    dx = torch.empty(dy.shape[:-1] + (K,), dtype=dy.dtype, device=dy.device)
+    dx = torch.empty(dy.shape[:-1] + (K,), dtype=dy.dtype, device=dev)
     dgate, dup = torch.empty_like(dy), torch.empty_like(dy)
     L = lib()
-    _i8_call(L.mi_int8_gate_up_swiglu_backward, dy.device,
-             L.mi_int8_backward_workspace(M, N, K, 2, code), _at(dx), _at(dgate), _at(dup),
-             _at(dy), _at(gate), _at(up), _at(wg), _at(sg), _at(wu), _at(su), M, N, K, code)
+    _i8_call(L.mi_int8_gate_up_swiglu_backward, dev, L.mi_int8_backward_workspace(M, N, K, 2, code), dx.data_ptr(),
+             dgate.data_ptr(), dup.data_ptr(), dy.data_ptr(), gate.data_ptr(), up.data_ptr(), wg.data_ptr(),
+             sg.data_ptr(), wu.data_ptr(), su.data_ptr(), M, N, K, code)
     return dx, dgate, dup
 
 
