@@ -107,6 +107,7 @@ int forward(mi::Int8Params& P, const void* x, const float* x_scales, int64_t M, 
   P.part = (int32_t*)((char*)ws + quant_bytes(M, K, x_dtype));
   const int a4 = P.type == mi::kF32 ? 16 : 8;
   P.vec = N % 4 == 0 && aligned(P.y, a4) && aligned(P.gate, a4) && aligned(P.up, a4);
+  P.vec16 = N % (P.type == mi::kF32 ? 4 : 8) == 0 && aligned(P.y, 16) && aligned(P.gate, 16) && aligned(P.up, 16);
   P.M = (int)M;
   P.N = (int)N;
   P.K = (int)K;
@@ -177,6 +178,7 @@ int backward(mi::Int8GradParams& G, mi::Int8BwdParams& B, int64_t M, int64_t N, 
   G.vec = N % (type == mi::kF32 ? 4 : 8) == 0 && aligned(G.dy, 16) && aligned(G.gate, 16) && aligned(G.up, 16) &&
           aligned(G.dgate, 16) && aligned(G.dup, 16) && aligned(G.sw, 16) && aligned(G.sw2, 16);
   B.vec = K % 4 == 0 && aligned(B.dx, type == mi::kF32 ? 16 : 8);
+  B.vec16 = K % (type == mi::kF32 ? 4 : 8) == 0 && aligned(B.dx, 16);
   const hipError_t e = mi::launch_int8_grad(G, s);
   if (e != hipSuccess) return hip_status(e, "int8 gradient launch");
   return hip_status(mi::int8_bwd_supported(K, B.w[0], B.w[1]) ? mi::launch_int8_bwd(B, s)

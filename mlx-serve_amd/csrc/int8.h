@@ -37,7 +37,8 @@ struct Int8Params {
   int bm, bn, ks, sps;
   int32_t* part;
   int nt;    // int8_gemv.hip: 16-row tiles of a wave; 0: another kernel
-  bool vec;  // y, gate, up, part rows of four columns on one store (N and pointers)
+  bool vec;    // four columns of y, gate and up with one store (N and pointers)
+  bool vec16;  // their rows on 16 bytes
 };
 
 // dx[m,k] = row[m] * sum over banks, parts and n of a[m,n] w[n,k]: the scaled gradients a as fp16,
@@ -53,7 +54,7 @@ struct Int8BwdParams {
   int M, N, K;
   int type;
   int bm, bn, ks, sps;  // int8_bwd.hip: rows and columns of a tile, ranges of sps 64-value steps over the parts
-  bool vec;
+  bool vec, vec16;      // as in Int8Params
 };
 
 // a = dy * sw[n] (one bank), or the two products of the SwiGLU gradient with sw / sw2.
@@ -233,10 +234,8 @@ MI_DEV Cols load_cols(const Int8Params& P, int n) {
 // The sums of columns n .. n + 3 (those below N) of row m, to memory: scales in 32 bits, one
 // rounding at the end.
 template <bool DUAL>
-MI_DEV void finish4(const Int8Params& P, int64_t m, int n, i32x4_t a, i32x4_t b, float sx, const Cols& c) {
-  const int64_t i = m * P.N + n;
-  const int cnt = P.N - n;
-  float y[4], u[4], g[4];
+MI_DEV void scaled4(const Int8Params& P, i32x4_t a, i32x4_t b, float sx, const Cols& c, float (&y)[4],
+                    float (&g)[4], float (&u)[4]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     g[j] = (float)a[j] * sx * c.s[j];
@@ -247,6 +246,13 @@ MI_DEV void finish4(const Int8Params& P, int64_t m, int n, i32x4_t a, i32x4_t b,
       y[j] = P.bias ? g[j] + c.b[j] : g[j];
     }
   }
+}
+template <bool DUAL>
+MI_DEV void finish4(const Int8Params& P, int64_t m, int n, i32x4_t a, i32x4_t b, float sx, const Cols& c) {
+  const int64_t i = m * P.N + n;
+  const int cnt = P.N - n;
+  float y[4], u[4], g[4];
+  scaled4<DUAL>(P, a, b, sx, c, y, g, u);
   store4(P.y, i, P.type, P.vec, cnt, y);
   if constexpr (DUAL) {
     if (P.gate) {

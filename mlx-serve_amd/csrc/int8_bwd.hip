@@ -225,23 +225,38 @@ int8_bwd_kernel(Int8BwdParams P) {
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // no DMA may outlive the block
 
   // acc[a][i] register j is [k = 16 (wn NT + a) + 4q + j][m = 16 (wm MT + i) + fr]
+  const int mw = m0 + 16 * wm * MT + fr, kw = k0 + 16 * wn * NT + 4 * q;
+  if constexpr (SPLIT) {
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int m = m0 + 16 * (wm * MT + i) + fr;
-    if (m >= M) continue;
-    const float row = P.row[m];
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int a = 0; a < NT; ++a) {
-      const int k = k0 + 16 * (wn * NT + a) + 4 * q;
-      if (k >= K) continue;  // K is a multiple of 16
-      const f32x4_t v = acc[a][i];
-      if constexpr (SPLIT) {
-        *reinterpret_cast<f32x4_t*>(P.part + ((size_t)at.split * M + m) * K + k) = v;
-      } else {
-        const float o[4] = {v[0] * row, v[1] * row, v[2] * row, v[3] * row};
-        store4(P.dx, (int64_t)m * K + k, P.type, P.vec, 4, o);
+      for (int a = 0; a < NT; ++a)
+        if (mw + 16 * i < M && kw + 16 * a < K)  // K is a multiple of 16
+          *reinterpret_cast<f32x4_t*>(P.part + ((size_t)at.split * M + mw + 16 * i) * K + kw + 16 * a) = acc[a][i];
+    return;
+  }
+  float row[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) row[i] = P.row[min(mw + 16 * i, M - 1)];
+  auto values = [&](int i, int a, float (&v)[1][4]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[0][j] = acc[a][i][j] * row[i];
+  };
+  void* const out[1] = {P.dx};
+  if (P.vec16 && P.type == kF32) {
+    store_tile<4, MT, NT, 1, lds_bytes<BM, BN, R>()>(smem, out, P.type, M, K, m0, k0, values);
+  } else if (P.vec16) {
+    store_tile<2, MT, NT, 1, lds_bytes<BM, BN, R>()>(smem, out, P.type, M, K, m0, k0, values);
+  } else {
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int a = 0; a < NT; ++a) {
+        float v[1][4];
+        values(i, a, v);
+        if (mw + 16 * i < M && kw + 16 * a < K)
+          store4(P.dx, (int64_t)(mw + 16 * i) * K + kw + 16 * a, P.type, P.vec, 4, v[0]);
       }
-    }
   }
 }
 

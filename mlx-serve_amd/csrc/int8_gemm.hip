@@ -24,6 +24,7 @@
 // K: any multiple of 16. In the last step the slots from K on load out of bounds, as zeros.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "int8_stage.h"
 #include "prefill_tiles.h"
@@ -171,25 +172,57 @@ int8_gemm_kernel(Int8Params P) {
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // no DMA may outlive the block
 
   // acc[a][i] register j is [n = 16 (wn NT + a) + 4q + j][m = 16 (wm MT + i) + fr]
-  const int mw = m0 + 16 * wm * MT + fr;
+  constexpr int TA = DUAL ? NT / 2 : NT;  // 16-column tiles of y
+  const int mw = m0 + 16 * wm * MT + fr, nw = n0 + 16 * wn * TA + 4 * q;
+  if constexpr (SPLIT) {
+#pragma unroll
+    for (int a = 0; a < TA; ++a)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+        if (nw + 16 * a < N && mw + 16 * i < M)
+          store_part<DUAL>(P, at.split, mw + 16 * i, nw + 16 * a, acc[DUAL ? 2 * a : a][i], acc[DUAL ? 2 * a + 1 : a][i]);
+    return;
+  }
   float sx[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) sx[i] = P.sx[min(mw + 16 * i, M - 1)];
+  Cols cols[TA];
 #pragma unroll
-  for (int a = 0; a < NT; a += DUAL ? 2 : 1) {
-    const int n = n0 + 16 * (DUAL ? (wn * NT + a) / 2 : wn * NT + a) + 4 * q;
-    if (n >= N) continue;
-    const Cols c = load_cols<DUAL>(P, n);
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const int m = mw + 16 * i;
-      if (m >= M) continue;
-      if constexpr (SPLIT)
-        store_part<DUAL>(P, at.split, m, n, acc[a][i], acc[DUAL ? a + 1 : a][i]);
-      else
-        finish4<DUAL>(P, m, n, acc[a][i], acc[DUAL ? a + 1 : a][i], sx[i], c);
-    }
+  for (int a = 0; a < TA; ++a) cols[a] = load_cols<DUAL>(P, min(nw + 16 * a, N - 1));
+  if (P.vec16) {
+    auto emit = [&](auto esz) __attribute__((always_inline)) {
+      constexpr int E = decltype(esz)::value;
+      auto values = [&](int i, int a, float (&y)[4], float (&g)[4], float (&u)[4]) __attribute__((always_inline)) {
+        scaled4<DUAL>(P, acc[DUAL ? 2 * a : a][i], acc[DUAL ? 2 * a + 1 : a][i], sx[i], cols[a], y, g, u);
+      };
+      if constexpr (DUAL) {
+        if (P.gate) {
+          void* const out[3] = {P.y, P.gate, P.up};
+          store_tile<E, MT, TA, 3, lds_bytes<BM, BN, R>()>(
+              smem, out, P.type, M, N, m0, n0,
+              [&](int i, int a, float (&v)[3][4]) __attribute__((always_inline)) { values(i, a, v[0], v[1], v[2]); });
+          return;
+        }
+      }
+      void* const out[1] = {P.y};
+      store_tile<E, MT, TA, 1, lds_bytes<BM, BN, R>()>(
+          smem, out, P.type, M, N, m0, n0, [&](int i, int a, float (&v)[1][4]) __attribute__((always_inline)) {
+            float g[4], u[4];
+            values(i, a, v[0], g, u);
+          });
+    };
+    if (P.type == kF32)
+      emit(std::integral_constant<int, 4>{});
+    else
+      emit(std::integral_constant<int, 2>{});
+    return;
   }
+#pragma unroll
+  for (int a = 0; a < TA; ++a)
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+      if (nw + 16 * a < N && mw + 16 * i < M)
+        finish4<DUAL>(P, mw + 16 * i, nw + 16 * a, acc[DUAL ? 2 * a : a][i], acc[DUAL ? 2 * a + 1 : a][i], sx[i], cols[a]);
 }
 
 // The splits' sums, exact in any order, and the scales.

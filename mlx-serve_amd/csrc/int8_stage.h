@@ -39,6 +39,59 @@ MI_DEV void wait_vm(int n) {
 }
 
 
+// A block's finished tile to memory through LDS, in rows of COLS values of ESZ bytes: stored straight
+// from the products' layout, a wave writes 32 bytes of each of 16 rows at a time, and a gate + up
+// tile with its two projections took 14 us to leave. Waves 2 x 4 with MT tiles of 16 rows and
+// TA tiles of 16 columns each; value(i, a, v) gives OUT x 4 values of the lane's row and columns.
+// Passes of 32 IC rows, so that OUT of them fit the staging LDS (its DMA has landed and its reads
+// are done, in every wave, after the first barrier). Rows of `out` on 16 bytes.
+template <int ESZ, int MT, int TA, int OUT, int LDS, class V>
+MI_DEV void store_tile(unsigned char* smem, void* const (&out)[OUT], int type, int M, int N, int m0, int n0,
+                       V value) {
+  constexpr int IC = MT < 8 / ESZ ? MT : 8 / ESZ;  // 4 (16-bit) or 2
+  constexpr int kCols = 64 * TA, kPitch = kCols * ESZ + 16, kRows = 32 * IC;
+  constexpr int kChunks = kCols * ESZ / 16;
+  static_assert(OUT * kRows * kPitch <= LDS && kRows * kChunks % 512 == 0 && MT % IC == 0, "a pass fits");
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int wm = wave >> 2, wn = wave & 3, fr = lane & 15, q = lane >> 4;
+#pragma unroll
+  for (int i0 = 0; i0 < MT; i0 += IC) {
+    lds_sync();
+#pragma unroll
+    for (int i = 0; i < IC; ++i)
+#pragma unroll
+      for (int a = 0; a < TA; ++a) {
+        float v[OUT][4];
+        value(i0 + i, a, v);
+#pragma unroll
+        for (int o = 0; o < OUT; ++o) {
+          unsigned char* p = smem + (o * kRows + 16 * (wm * IC + i) + fr) * kPitch + (16 * (wn * TA + a) + 4 * q) * ESZ;
+          if constexpr (ESZ == 4) {
+            *reinterpret_cast<f32x4_t*>(p) = f32x4_t{v[o][0], v[o][1], v[o][2], v[o][3]};
+          } else {
+            uint32_t b[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              b[j] = type == kBF16 ? f32_to_bf16_bits(v[o][j])
+                                   : (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[o][j]);
+            *reinterpret_cast<u32x2_t*>(p) = u32x2_t{b[0] | b[1] << 16, b[2] | b[3] << 16};
+          }
+        }
+      }
+    lds_sync();
+#pragma unroll
+    for (int o = 0; o < OUT; ++o)
+#pragma unroll
+      for (int k = 0; k < kRows * kChunks / 512; ++k) {
+        const int at = tid + 512 * k, r = at / kChunks, c = at % kChunks;
+        const int m = m0 + 16 * (r / (16 * IC) * MT + i0 + r / 16 % IC) + r % 16, n = n0 + c * (16 / ESZ);
+        if (m < M && n < N)
+          *reinterpret_cast<u32x4_t*>((unsigned char*)out[o] + ((int64_t)m * N + n) * ESZ) =
+              *reinterpret_cast<const u32x4_t*>(smem + (o * kRows + r) * kPitch + c * 16);
+      }
+  }
+}
+
 // A tile of the matrix kernels for their plans: microseconds a step of a block that has its CU to
 // itself, of two that share it (0: a block fills the CU), and beside the steps (start, end).
 struct TileCost {
