@@ -35,6 +35,8 @@ struct Int8Params {
   // int8_gemm.hip: rows of x and of w (both banks) of a tile; K ranges over blocks and 128-code steps of one, ks > 1
   // through int32 sums [ks][banks][M][N] in `part`
   int bm, bn, ks, sps;
+  int ct0, ct1;  // column tiles of a launch
+  int tail;      // 256 x 256 tiles: column tiles at the end that 128 x 256 ones take, in a launch of their own
   int32_t* part;
   int nt;    // int8_gemv.hip: 16-row tiles of a wave; 0: another kernel
   bool vec;    // four columns of y, gate and up with one store (N and pointers)
@@ -54,7 +56,8 @@ struct Int8BwdParams {
   int M, N, K;
   int type;
   int bm, bn, ks, sps;  // int8_bwd.hip: rows and columns of a tile, ranges of sps 64-value steps over the parts
-  bool vec, vec16;      // as in Int8Params
+  int ct0, ct1, tail;   // as in Int8Params
+  bool vec, vec16;
 };
 
 // a = dy * sw[n] (one bank), or the two products of the SwiGLU gradient with sw / sw2.

@@ -69,8 +69,8 @@ int8_bwd_kernel(Int8BwdParams P) {
   const int fr = lane & 15, q = lane >> 4;
   const int M = P.M, N = P.N, K = P.K, np = P.np;
   const int mtiles = (M + BM - 1) / BM;
-  const TileOf at = tile_of_block(mtiles, (K + BN - 1) / BN);
-  const int m0 = at.mt * BM, k0 = at.nt * BN, s0 = at.split * P.sps;
+  const TileOf at = tile_of_block(mtiles, P.ct1 - P.ct0);
+  const int m0 = at.mt * BM, k0 = (P.ct0 + at.nt) * BN, s0 = at.split * P.sps;
   const int seg_steps = np / kBN_;
   const int ns = min(P.sps, P.banks * P.terms * seg_steps - s0);
   const int mrows = min(BM, M - m0);
@@ -286,7 +286,7 @@ hipError_t launch_tile(const Int8BwdParams& P, hipStream_t s) {
     if (e == hipSuccess) done |= bit;
   }
   if (e != hipSuccess) return e;
-  const dim3 grid((unsigned)(((P.M + BM - 1) / BM) * ((P.K + BN - 1) / BN)), (unsigned)P.ks);
+  const dim3 grid((unsigned)(((P.M + BM - 1) / BM) * (P.ct1 - P.ct0)), (unsigned)P.ks);
   if (P.ks > 1)
     hipLaunchKernelGGL((int8_bwd_kernel<BM, BN, R, true>), grid, dim3(512), lds, s, P);
   else
@@ -315,23 +315,33 @@ void int8_bwd_plan(Int8BwdParams& P) {
     for (int k = 1; k <= std::max(1, steps / 4) && k <= 64; ++k) {
       const int sps = (steps + k - 1) / k, ks = (steps + sps - 1) / sps;
       const double part = ks > 1 ? (double)ks * P.M * P.K * 8 / 5e6 + 3.0 : 0.0;
-      const double cost = tile_us(t, tiles * ks, sps) + part;
+      double cost = tile_us(t, tiles * ks, sps) + part;
+      const int tail = t.bm == 256 && ks == 1 ? tail_columns(t, kTiles[1], P.M, (P.K + 255) / 256, steps, &cost) : 0;
       if (cost < best - 1e-9) {
         best = cost;
         P.bm = t.bm;
         P.bn = t.bn;
         P.ks = ks;
         P.sps = sps;
+        P.tail = tail;
       }
     }
   }
 }
 
-hipError_t launch_int8_bwd(const Int8BwdParams& P, hipStream_t s) {
-  const hipError_t e = P.bm == 256   ? launch_tile<256, 256, 3>(P, s)
-                       : P.bm == 128 ? (P.bn == 256 ? launch_tile<128, 256, 4>(P, s)
-                                                    : launch_tile<128, 128, 3>(P, s))
-                                     : launch_tile<64, 128, 4>(P, s);
+hipError_t launch_int8_bwd(const Int8BwdParams& given, hipStream_t s) {
+  Int8BwdParams P = given;
+  const int ct = (P.K + P.bn - 1) / P.bn;
+  P.ct0 = 0;
+  P.ct1 = ct - P.tail;
+  hipError_t e = P.bm == 256   ? launch_tile<256, 256, 3>(P, s)
+                 : P.bm == 128 ? (P.bn == 256 ? launch_tile<128, 256, 4>(P, s) : launch_tile<128, 128, 3>(P, s))
+                               : launch_tile<64, 128, 4>(P, s);
+  if (e == hipSuccess && P.tail) {
+    P.ct0 = P.ct1;
+    P.ct1 = ct;
+    e = launch_tile<128, 256, 4>(P, s);
+  }
   if (e != hipSuccess || P.ks == 1) return e;
   int64_t g = ((int64_t)P.M * P.K / 4 + 255) / 256;
   if (g > 8192) g = 8192;

@@ -56,8 +56,8 @@ int8_gemm_kernel(Int8Params P) {
   const int fr = lane & 15, q = lane >> 4;
   const int M = P.M, N = P.N, K = P.K, ldx = (int)P.ldx;
   const int mtiles = (M + BM - 1) / BM;
-  const TileOf at = tile_of_block(mtiles, (N + kON - 1) / kON);
-  const int m0 = at.mt * BM, n0 = at.nt * kON, s0 = at.split * P.sps;
+  const TileOf at = tile_of_block(mtiles, P.ct1 - P.ct0);
+  const int m0 = at.mt * BM, n0 = (P.ct0 + at.nt) * kON, s0 = at.split * P.sps;
   const int ns = min(P.sps, (K + kBK - 1) / kBK - s0);
   const int mrows = min(BM, M - m0), nrows = min(kON, N - n0);
   const int xbytes = mrows * ldx, wbytes = nrows * K;
@@ -244,7 +244,6 @@ __global__ void __launch_bounds__(256) int8_reduce_kernel(Int8Params P) {
 template <bool DUAL, int BM, int BN, int R>
 hipError_t launch_tile(const Int8Params& P, hipStream_t s) {
   constexpr int lds = lds_bytes<BM, BN, R>();
-  constexpr int kON = DUAL ? BN / 2 : BN;
   static std::atomic<uint64_t> done{0};  // devices whose functions have the attribute
   int dev = 0;
   hipError_t e = hipGetDevice(&dev);
@@ -256,7 +255,7 @@ hipError_t launch_tile(const Int8Params& P, hipStream_t s) {
     if (e == hipSuccess) done |= bit;
   }
   if (e != hipSuccess) return e;
-  const dim3 grid((unsigned)(((P.M + BM - 1) / BM) * ((P.N + kON - 1) / kON)), (unsigned)P.ks);
+  const dim3 grid((unsigned)(((P.M + BM - 1) / BM) * (P.ct1 - P.ct0)), (unsigned)P.ks);
   if (P.ks > 1)
     hipLaunchKernelGGL((int8_gemm_kernel<DUAL, BM, BN, R, true>), grid, dim3(512), lds, s, P);
   else
@@ -265,11 +264,19 @@ hipError_t launch_tile(const Int8Params& P, hipStream_t s) {
 }
 
 template <bool DUAL>
-hipError_t launch_gemm(const Int8Params& P, hipStream_t s) {
+hipError_t launch_gemm(Int8Params P, hipStream_t s) {
+  const int cols = DUAL ? P.bn / 2 : P.bn, ct = (P.N + cols - 1) / cols;
+  P.ct0 = 0;
+  P.ct1 = ct - P.tail;
   hipError_t e = P.bm == 256   ? launch_tile<DUAL, 256, 256, 2>(P, s)
                  : P.bm == 128 ? (P.bn == 256 ? launch_tile<DUAL, 128, 256, 3>(P, s)
                                               : launch_tile<DUAL, 128, 128, 2>(P, s))
                                : launch_tile<DUAL, 64, 128, 3>(P, s);
+  if (e == hipSuccess && P.tail) {
+    P.ct0 = P.ct1;
+    P.ct1 = ct;
+    e = launch_tile<DUAL, 128, 256, 3>(P, s);
+  }
   if (e != hipSuccess || P.ks == 1) return e;
   int64_t g = ((int64_t)P.M * ((P.N + 3) / 4) + 255) / 256;
   if (g > 8192) g = 8192;
@@ -298,13 +305,15 @@ double int8_gemm_plan(Int8Params& P) {
     for (int k = 1; k <= std::max(1, steps / 4) && k <= 64; ++k) {
       const int sps = (steps + k - 1) / k, ks = (steps + sps - 1) / sps;
       const double part = ks > 1 ? (double)ks * banks * P.M * P.N * 8 / 5e6 + 3.0 : 0.0;
-      const double cost = tile_us(t, tiles * ks, sps) + part;
+      double cost = tile_us(t, tiles * ks, sps) + part;
+      const int tail = t.bm == 256 && ks == 1 ? tail_columns(t, kTiles[1], P.M, (P.N + on - 1) / on, steps, &cost) : 0;
       if (cost < best - 1e-9) {
         best = cost;
         P.bm = t.bm;
         P.bn = t.bn;
         P.ks = ks;
         P.sps = sps;
+        P.tail = tail;
       }
     }
   }

@@ -106,5 +106,18 @@ inline double tile_us(const TileCost& t, int64_t tiles, int steps) {
   return (double)(per_cu / 2) * (steps * t.paired + t.ends) + (per_cu % 2 ? one : 0.0);
 }
 
+// Whole rounds of big tiles and, for what is left of the last one, small tiles in a launch of their own:
+// the column tiles at the end that those take, 0 where it would not pay. `ct` column tiles of `big`
+// (256 rows) and `small` (128) alike.
+inline int tail_columns(const TileCost& big, const TileCost& small, int64_t M, int64_t ct, int steps, double* us) {
+  const int64_t bt = (M + 255) / 256, st = (M + 127) / 128, rounds = bt * ct / 256;
+  if (rounds < 1 || bt * ct % 256 == 0 || bt > 256) return 0;
+  const int64_t tail = ct - rounds * 256 / bt;
+  const double cost = tile_us(big, bt * (ct - tail), steps) + tile_us(small, st * tail, steps) + 2.0;
+  if (cost >= *us) return 0;
+  *us = cost;
+  return (int)tail;
+}
+
 }  // namespace i8
 }  // namespace mi

@@ -214,7 +214,68 @@ def test_unaligned_pointers(dev, M):
     R.check(dx, *R.matmul_backward(dy, w, sw), "aligned")
 
 
+# Sizes that reach every tile, its splits of K and the small tiles behind whole rounds of big ones; K ends
+# inside a step (a multiple of 16 only), rows and columns inside tiles.
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("M,N,K", [(1100, 9000, 2064), (2600, 7700, 2064), (2600, 7701, 1040), (600, 5002, 2064),
+                                   (1300, 2000, 1040), (300, 1000, 4112), (600, 1001, 8208), (150, 700, 8208),
+                                   (129, 24, 16400), (257, 4104, 16)])
+def test_matmul_tiles(dev, M, N, K, t):
+    _case(t="matmul_tiles", M=M, N=N, K=K, type=t)
+    g = _gen(M + N)
+    w, sw = _weights(g, N, K)
+    x = _x(g, M, K, t)
+    q, sx = mi_qmm.int8_quantize(x)
+    b = _x(g, 1, N, t)[0]
+    ref, tol = R.matmul(q, sx, w, sw, b)
+    y = mi_qmm.int8_matmul(x, w, sw, bias=b)
+    R.check(y, ref, tol(t), "y")
+    assert torch.equal(y, mi_qmm.int8_matmul(x, w, sw, bias=b))
+
+
+@pytest.mark.parametrize("t,save", [(BF16, True), (F16, False), (F32, True)])
+@pytest.mark.parametrize("M,N,K", [(1100, 4500, 2064), (1300, 13000, 1040), (600, 2501, 2064), (300, 1000, 4112),
+                                   (600, 1000, 8208), (150, 350, 8208), (700, 10000, 528)])
+def test_gate_up_tiles(dev, M, N, K, t, save):
+    _case(t="gate_up_tiles", M=M, N=N, K=K, type=t)
+    g = _gen(M + N)
+    (wg, sg), (wu, su) = _weights(g, N, K), _weights(g, N, K)
+    x = _x(g, M, K, t)
+    q, sx = mi_qmm.int8_quantize(x)
+    y, gate, up, ty, tg, tu = R.gate_up(q, sx, wg, sg, wu, su)
+    o = mi_qmm.int8_gate_up_swiglu(x, wg, sg, wu, su, save=save)
+    for a, b, tol in zip(o if save else (o,), (y, gate, up), (ty, tg, tu)):
+        R.check(a, b, tol(t), "saved")
+
+
 # ------------------------------------------------------------------- gradients --
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("M,K,N", [(520, 32992, 130), (1100, 9008, 2050), (2600, 7696, 1026), (600, 5008, 2050),
+                                   (130, 5008, 2050), (300, 1008, 4100), (600, 1008, 8200), (70, 528, 8200),
+                                   (257, 16, 2049)])
+def test_matmul_backward_tiles(dev, M, K, N, t):
+    _case(t="matmul_bwd_tiles", M=M, N=N, K=K, type=t)
+    g = _gen(M + N)
+    w, sw = _weights(g, N, K)
+    dy = _x(g, M, N, t)
+    dx = mi_qmm.int8_matmul_backward(dy, w, sw)
+    R.check(dx, *R.matmul_backward(dy, w, sw), "dx")
+    assert torch.equal(dx, mi_qmm.int8_matmul_backward(dy, w, sw))
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("M,K,N", [(1100, 9008, 520), (2600, 7696, 514), (130, 1008, 2050), (300, 2000, 14336)])
+def test_gate_up_backward_tiles(dev, M, K, N, t):
+    _case(t="gate_up_bwd_tiles", M=M, N=N, K=K, type=t)
+    g = _gen(M + N)
+    (wg, sg), (wu, su) = _weights(g, N, K), _weights(g, N, K)
+    dy, gate, up = _x(g, M, N, t), _x(g, M, N, t) * 2, _x(g, M, N, t)
+    ref, tol = R.gate_up_backward(dy, gate, up, wg, sg, wu, su)
+    for a, r, e, what in zip(mi_qmm.int8_gate_up_swiglu_backward(dy, gate, up, wg, sg, wu, su), ref, tol,
+                             ("dx", "dgate", "dup")):
+        R.check(a, r, e, what)
+
+
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("N,K", [(1, 1), (16, 64), (33, 208), (130, 77), (64, 4096), (1536, 520), (2052, 132)])
 @pytest.mark.parametrize("M", [1, 2, 17, 64, 65, 129, 300])
