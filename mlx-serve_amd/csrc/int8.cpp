@@ -51,13 +51,15 @@ int check_workspace(const void* ws, int64_t given, int64_t need) {
   return MI_OK;
 }
 
-// Forward workspace: codes [M, ldx] and scales of activations that come as floats, then the K
-// ranges' sums of a split product. Sizes alone decide what is asked for; a call on pointers
-// that another kernel has to take leaves the sums' part unused.
-int64_t codes_bytes(int64_t M, int64_t K) { return up(M * up(K, 16), 256); }
-int64_t quant_bytes(int64_t M, int64_t K, int x_dtype) {
-  return x_dtype == MI_DTYPE_INT8 ? 0 : codes_bytes(M, K) + up(M * 4, 256);
+// Forward workspace: codes [M, ld] and scales of activations that come as floats; where K is no
+// multiple of 16 also rows of ld = K rounded up for x and w; then the K ranges' sums of a split
+// product. Sizes alone decide what is asked for; a call on pointers that another kernel has to
+// take leaves the sums' part unused.
+int64_t x_bytes(int64_t M, int64_t K, int x_dtype) {
+  return x_dtype == MI_DTYPE_INT8 && K % 16 == 0 ? 0 : up(M * up(K, 16), 256);
 }
+int64_t sx_bytes(int64_t M, int x_dtype) { return x_dtype == MI_DTYPE_INT8 ? 0 : up(M * 4, 256); }
+int64_t w_bytes(int64_t N, int64_t K) { return K % 16 == 0 ? 0 : up(N * up(K, 16), 256); }  // a bank
 bool fused_token(int64_t M, int64_t K, int x_dtype) {
   return x_dtype != MI_DTYPE_INT8 && mi::int8_gemv_fuses(M, K, float_type(x_dtype));
 }
@@ -65,25 +67,22 @@ int64_t forward_need(mi::Int8Params& P, int64_t M, int64_t N, int64_t K, int x_d
   if (M == 0 || N == 0 || K == 0 || fused_token(M, K, x_dtype)) return 0;
   P.M = (int)M;
   P.N = (int)N;
-  P.K = (int)K;
+  P.K = (int)up(K, 16);
   P.ks = 1;
-  P.nt = 0;
-  if (K % 16 == 0) {  // up to 16 rows the few-row kernel, up to 128 the one that should be faster
-    const double few = M <= mi::kInt8FewRows ? mi::int8_gemv_plan(P) : 0.0;
-    const int nt = P.nt;
-    const double tiles = M > 16 ? mi::int8_gemm_plan(P) : 0.0;
-    if (nt && M > 16 && tiles < few) P.nt = 0;
-    if (P.nt) P.ks = 1;
-  }
-  return quant_bytes(M, K, x_dtype) + (P.ks > 1 ? (int64_t)P.ks * P.banks * M * N * 4 : 0);
-}
-// Blocks of a launch, below 2^32 threads.
-bool forward_fits(int64_t M, int64_t N) {
-  return ((M + 63) / 64) * ((N + 63) / 64) <= kMaxTiles && (M > mi::kInt8FewRows || N <= (int64_t)1 << 26);
+  // up to 16 rows the few-row kernel, up to 128 the one that should be faster
+  const double few = M <= mi::kInt8FewRows ? mi::int8_gemv_plan(P) : (P.nt = 0, 0.0);
+  if (M > 16 && mi::int8_gemm_plan(P) < few) P.nt = 0;
+  if (P.nt) P.ks = 1;
+  return x_bytes(M, K, x_dtype) + sx_bytes(M, x_dtype) + P.banks * w_bytes(N, K) +
+         (P.ks > 1 ? (int64_t)P.ks * P.banks * M * N * 4 : 0);
 }
 bool aligned(const void* p, int a) { return (uintptr_t)p % a == 0; }
 bool rows_on_16(const mi::Int8Params& P) {
   return ((uintptr_t)P.x | (uintptr_t)P.ldx | (uintptr_t)P.w | (uintptr_t)P.w2 | (uintptr_t)P.K) % 16 == 0;
+}
+// Blocks of a launch, below 2^32 threads.
+bool forward_fits(int64_t M, int64_t N) {
+  return ((M + 63) / 64) * ((N + 63) / 64) <= kMaxTiles && (M > mi::kInt8FewRows || N <= (int64_t)1 << 26);
 }
 
 int forward(mi::Int8Params& P, const void* x, const float* x_scales, int64_t M, int64_t N,
@@ -104,7 +103,6 @@ int forward(mi::Int8Params& P, const void* x, const float* x_scales, int64_t M, 
   P.banks = P.w2 ? 2 : 1;
   const int64_t need = forward_need(P, M, N, K, x_dtype);
   if (int rc = check_workspace(ws, ws_bytes, need)) return rc;
-  P.part = (int32_t*)((char*)ws + quant_bytes(M, K, x_dtype));
   const int a4 = P.type == mi::kF32 ? 16 : 8;
   P.vec = N % 4 == 0 && aligned(P.y, a4) && aligned(P.gate, a4) && aligned(P.up, a4);
   P.vec16 = N % (P.type == mi::kF32 ? 4 : 8) == 0 && aligned(P.y, 16) && aligned(P.gate, 16) && aligned(P.up, 16);
@@ -120,21 +118,40 @@ int forward(mi::Int8Params& P, const void* x, const float* x_scales, int64_t M, 
     return hip_status(rows_on_16(P) ? mi::launch_int8_gemv(P, s) : mi::launch_int8_any(P, s),
                       "int8 matmul launch");
   }
+  const int64_t ld = up(K, 16);
+  char* at = (char*)ws;
+  hipError_t e = hipSuccess;
   if (xt >= 0) {
-    P.ldx = up(K, 16);
-    P.x = (const int8_t*)ws;
-    P.sx = (const float*)((char*)ws + codes_bytes(M, K));
-    const hipError_t e = mi::launch_int8_quantize((int8_t*)ws, (float*)P.sx, x, M, K, P.ldx, xt, s);
-    if (e != hipSuccess) return hip_status(e, "int8 quantize launch");
+    P.x = (const int8_t*)at;
+    P.sx = (const float*)(at + x_bytes(M, K, x_dtype));
+    P.ldx = ld;
+    e = mi::launch_int8_quantize((int8_t*)at, (float*)P.sx, x, M, K, ld, xt, s);
+  } else if (ld != K) {
+    P.x = (const int8_t*)at;
+    P.ldx = ld;
+    e = mi::launch_int8_pad((int8_t*)at, (const int8_t*)x, M, K, ld, s);
   }
+  at += x_bytes(M, K, x_dtype) + sx_bytes(M, x_dtype);
+  if (ld != K) {
+    P.K = (int)ld;  // the zeros behind K add nothing
+    for (const int8_t** w : {&P.w, &P.w2}) {
+      if (e != hipSuccess || !*w) continue;
+      e = mi::launch_int8_pad((int8_t*)at, *w, N, K, ld, s);
+      *w = (const int8_t*)at;
+      at += w_bytes(N, K);
+    }
+  }
+  P.part = (int32_t*)at;
+  if (e != hipSuccess) return hip_status(e, "int8 quantize launch");
   return hip_status(!rows_on_16(P) ? mi::launch_int8_any(P, s)
                     : P.nt         ? mi::launch_int8_gemv(P, s)
                                    : mi::launch_int8_gemm(P, s),
                     "int8 matmul launch");
 }
 
-// Backward workspace: the fp16 parts of the scaled gradients, [banks * terms][M][np], the rows'
-// powers of two, then the ranges' sums of a split product. Two parts for fp32, one otherwise.
+// Backward workspace: the fp16 parts of the scaled gradients, [banks * terms][M][np] (two parts for
+// fp32, one otherwise), the rows' powers of two, the codes in rows of ldw where K is no multiple of
+// 16, then the ranges' sums of a split product.
 int64_t parts_bytes(const mi::Int8BwdParams& B) { return up((int64_t)B.banks * B.terms * B.M * B.np * 2, 256); }
 int64_t rows_bytes(const mi::Int8BwdParams& B) { return up((int64_t)B.M * 4, 256); }
 int64_t backward_need(mi::Int8BwdParams& B, int64_t M, int64_t N, int64_t K, int banks, int type) {
@@ -145,10 +162,10 @@ int64_t backward_need(mi::Int8BwdParams& B, int64_t M, int64_t N, int64_t K, int
   B.M = (int)M;
   B.N = (int)N;
   B.K = (int)K;
+  B.ldw = (int)up(K, 16);
   B.type = type;
-  B.ks = 1;
-  if (K % 16 == 0) mi::int8_bwd_plan(B);
-  return parts_bytes(B) + rows_bytes(B) + (B.ks > 1 ? (int64_t)B.ks * M * K * 4 : 0);
+  mi::int8_bwd_plan(B);
+  return parts_bytes(B) + rows_bytes(B) + banks * w_bytes(N, K) + (B.ks > 1 ? (int64_t)B.ks * M * B.ldw * 4 : 0);
 }
 
 int backward(mi::Int8GradParams& G, mi::Int8BwdParams& B, int64_t M, int64_t N, int64_t K, int dtype,
@@ -168,7 +185,7 @@ int backward(mi::Int8GradParams& G, mi::Int8BwdParams& B, int64_t M, int64_t N, 
   G.row = (float*)((char*)ws + parts_bytes(B));
   B.a = G.a;
   B.row = G.row;
-  B.part = (float*)((char*)G.row + rows_bytes(B));
+  char* at = (char*)G.row + rows_bytes(B);
   G.banks = banks;
   G.terms = B.terms;
   G.np = B.np;
@@ -179,11 +196,16 @@ int backward(mi::Int8GradParams& G, mi::Int8BwdParams& B, int64_t M, int64_t N, 
           aligned(G.dgate, 16) && aligned(G.dup, 16) && aligned(G.sw, 16) && aligned(G.sw2, 16);
   B.vec = K % 4 == 0 && aligned(B.dx, type == mi::kF32 ? 16 : 8);
   B.vec16 = K % (type == mi::kF32 ? 4 : 8) == 0 && aligned(B.dx, 16);
-  const hipError_t e = mi::launch_int8_grad(G, s);
+  hipError_t e = mi::launch_int8_grad(G, s);
+  for (int b = 0; b < banks && B.ldw != K; ++b) {
+    if (e == hipSuccess) e = mi::launch_int8_pad((int8_t*)at, B.w[b], N, K, B.ldw, s);
+    B.w[b] = (const int8_t*)at;
+    at += w_bytes(N, K);
+  }
+  B.part = (float*)at;
   if (e != hipSuccess) return hip_status(e, "int8 gradient launch");
-  return hip_status(mi::int8_bwd_supported(K, B.w[0], B.w[1]) ? mi::launch_int8_bwd(B, s)
-                                                              : mi::launch_int8_bwd_any(B, s),
-                    "int8 backward launch");
+  const bool fast = ((uintptr_t)B.w[0] | (uintptr_t)B.w[1]) % 16 == 0;
+  return hip_status(fast ? mi::launch_int8_bwd(B, s) : mi::launch_int8_bwd_any(B, s), "int8 backward launch");
 }
 
 }  // namespace

@@ -49,11 +49,11 @@ struct Int8Params {
 struct Int8BwdParams {
   const uint16_t* a;
   const float* row;    // [M]
-  const int8_t* w[2];  // [N, K]
+  const int8_t* w[2];  // [N, ldw]
   void* dx;            // [M, K]
-  float* part;         // ks > 1: fp32 sums [ks][M][K]
+  float* part;         // ks > 1: fp32 sums [ks][M][ldw]
   int banks, terms, np;
-  int M, N, K;
+  int M, N, K, ldw;
   int type;
   int bm, bn, ks, sps;  // int8_bwd.hip: rows and columns of a tile, ranges of sps 64-value steps over the parts
   int ct0, ct1, tail;   // as in Int8Params
@@ -84,9 +84,9 @@ bool int8_gemv_fuses(int64_t M, int64_t K, int type);
 hipError_t launch_int8_gemv(const Int8Params& P, hipStream_t s);
 double int8_gemm_plan(Int8Params& P);  // bm, ks, sps, from the same; returns estimated us
 hipError_t launch_int8_gemm(const Int8Params& P, hipStream_t s);
+hipError_t launch_int8_pad(int8_t* to, const int8_t* from, int64_t rows, int64_t K, int64_t ld, hipStream_t s);
 hipError_t launch_int8_any(const Int8Params& P, hipStream_t s);
 hipError_t launch_int8_grad(const Int8GradParams& P, hipStream_t s);
-bool int8_bwd_supported(int64_t K, const void* w, const void* w2);
 void int8_bwd_plan(Int8BwdParams& P);  // from M, K, np, banks and terms: bm, bn, ks, sps
 hipError_t launch_int8_bwd(const Int8BwdParams& P, hipStream_t s);
 hipError_t launch_int8_bwd_any(const Int8BwdParams& P, hipStream_t s);

@@ -1,7 +1,8 @@
-// Int8 products of any size and alignment: 64 x 64 output tiles, operands staged through LDS byte
-// by byte where a 16-byte load could leave the row. The kernels of int8_gemv.hip, int8_gemm.hip and
-// int8_bwd.hip take the aligned layouts; what is left here are rows of K bytes that are no multiple
-// of 16, as no model's are.
+// Int8 products of any size and alignment: 64 x 64 output tiles, operands staged through LDS, byte by
+// byte where a 16-byte load could leave the row. The kernels of int8_gemv.hip, int8_gemm.hip and
+// int8_bwd.hip take rows on 16 bytes; what is left here are pointers that are not. (Rows of K bytes, no
+// multiple of 16, are first copied to such: int8_pad_kernel. Straight from them, 16 rows' gradient
+// through a [4001,1001] matrix took 188 us.)
 #include "int8.h"
 
 namespace mi {
@@ -12,14 +13,28 @@ using namespace i8;
 constexpr int kT = 64;        // rows of either operand
 constexpr int kLd = 64 + 16;  // bytes of a staged row: 16-byte aligned, banks spread
 
-// 16 codes k .. k+15 of a row, zeros from K on
-MI_DEV u32x4_t codes16(const int8_t* row, int k, int K, bool aligned) {
-  if (k + 16 <= K && aligned) return *reinterpret_cast<const u32x4_t*>(row + k);
+// 16 codes k .. k+15 of a row at any address, zeros from K on
+MI_DEV u32x4_t codes16(const int8_t* row, int k, int K) {
   u32x4_t v = {0, 0, 0, 0};
+  if (k + 16 <= K) {
+    __builtin_memcpy(&v, row + k, 16);
+    return v;
+  }
 #pragma unroll
   for (int j = 0; j < 16; ++j)
     if (k + j < K) v[j / 4] |= (uint32_t)(uint8_t)row[k + j] << (8 * (j % 4));
   return v;
+}
+
+// Rows of K codes to rows of ld, a multiple of 16, zeros from K on.
+__global__ void __launch_bounds__(256) int8_pad_kernel(int8_t* __restrict__ to, const int8_t* __restrict__ from,
+                                                       int64_t rows, int K, int ld) {
+  const int64_t per = ld / 16, total = rows * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / per;
+    const int k = (int)(i - r * per) * 16;
+    *reinterpret_cast<u32x4_t*>(to + r * ld + k) = codes16(from + r * K, k, K);
+  }
 }
 
 // y (or the gate and up products): block of 4 waves, wave w rows 16w .. 16w+15 of the weights
@@ -33,8 +48,6 @@ __global__ void __launch_bounds__(256) int8_any_kernel(Int8Params P) {
   const int ntiles = (P.N + kT - 1) / kT;
   const int64_t m0 = (int64_t)(blockIdx.x / ntiles) * kT;
   const int n0 = (int)(blockIdx.x % ntiles) * kT;
-  const bool xa = ((uintptr_t)P.x | (uintptr_t)P.ldx) % 16 == 0;
-  const bool wa = ((uintptr_t)P.w | (uintptr_t)(DUAL ? P.w2 : P.w) | (uintptr_t)P.K) % 16 == 0;
   const int r = tid >> 2, rb = 16 * (tid & 3);  // the row and bytes this thread stages
   const int64_t xm = min(m0 + r, (int64_t)P.M - 1);
   const int64_t wn = min(n0 + r, P.N - 1);
@@ -44,10 +57,10 @@ __global__ void __launch_bounds__(256) int8_any_kernel(Int8Params P) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[b][i] = i32x4_t{0, 0, 0, 0};
   for (int k = 0; k < P.K; k += 64) {
-    *reinterpret_cast<u32x4_t*>(xs + r * kLd + rb) = codes16(P.x + xm * P.ldx, k + rb, P.K, xa);
-    *reinterpret_cast<u32x4_t*>(ws + r * kLd + rb) = codes16(P.w + wn * P.K, k + rb, P.K, wa);
+    *reinterpret_cast<u32x4_t*>(xs + r * kLd + rb) = codes16(P.x + xm * P.ldx, k + rb, P.K);
+    *reinterpret_cast<u32x4_t*>(ws + r * kLd + rb) = codes16(P.w + wn * P.K, k + rb, P.K);
     if constexpr (DUAL)
-      *reinterpret_cast<u32x4_t*>(ws + (kT + r) * kLd + rb) = codes16(P.w2 + wn * P.K, k + rb, P.K, wa);
+      *reinterpret_cast<u32x4_t*>(ws + (kT + r) * kLd + rb) = codes16(P.w2 + wn * P.K, k + rb, P.K);
     __syncthreads();
 #pragma unroll
     for (int b = 0; b < (DUAL ? 2 : 1); ++b) {
@@ -175,6 +188,13 @@ hipError_t launch_bwd(const Int8BwdParams& P, hipStream_t s) {
 }
 
 }  // namespace
+
+hipError_t launch_int8_pad(int8_t* to, const int8_t* from, int64_t rows, int64_t K, int64_t ld, hipStream_t s) {
+  const int64_t blocks = (rows * (ld / 16) + 255) / 256;
+  hipLaunchKernelGGL(int8_pad_kernel, dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(256), 0, s, to, from,
+                     rows, (int)K, (int)ld);
+  return hipGetLastError();
+}
 
 hipError_t launch_int8_any(const Int8Params& P, hipStream_t s) {
   if (P.xf)

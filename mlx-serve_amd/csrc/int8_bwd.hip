@@ -67,7 +67,7 @@ int8_bwd_kernel(Int8BwdParams P) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave >> 2, wn = wave & 3;
   const int fr = lane & 15, q = lane >> 4;
-  const int M = P.M, N = P.N, K = P.K, np = P.np;
+  const int M = P.M, N = P.N, K = P.K, ldw = P.ldw, np = P.np;
   const int mtiles = (M + BM - 1) / BM;
   const TileOf at = tile_of_block(mtiles, P.ct1 - P.ct0);
   const int m0 = at.mt * BM, k0 = (P.ct0 + at.nt) * BN, s0 = at.split * P.sps;
@@ -87,7 +87,7 @@ int8_bwd_kernel(Int8BwdParams P) {
   for (int i = 0; i < WI; ++i) {
     wr[i] = kRI * (wave * WI + i) + lane / (BN / 16);
     const int c = 16 * ((lane % (BN / 16)) ^ nswz<BN>(wr[i]));
-    wo[i] = k0 + c < K ? (uint32_t)wr[i] * (uint32_t)K + (uint32_t)(k0 + c) : kOOB;
+    wo[i] = k0 + c < ldw ? (uint32_t)wr[i] * (uint32_t)ldw + (uint32_t)(k0 + c) : kOOB;
   }
   // where a stage reads: part `seg`, values n .. n + 63 of it
   struct Cursor {
@@ -106,7 +106,7 @@ int8_bwd_kernel(Int8BwdParams P) {
     }
   };
   auto abase = [&](const Cursor& c) { return P.a + ((size_t)c.seg * M + m0) * np; };
-  auto wbase = [&](const Cursor& c) { return P.w[c.seg >= P.terms] + (size_t)c.n * K; };
+  auto wbase = [&](const Cursor& c) { return P.w[c.seg >= P.terms] + (size_t)c.n * ldw; };
   // stages past the range load through resources of zero records (zeros, no traffic), rows from N
   // on and columns from K on out of bounds
   auto issue = [&](const Cursor& c, int slot, int j) __attribute__((always_inline)) {  // instruction j
@@ -116,21 +116,21 @@ int8_bwd_kernel(Int8BwdParams P) {
       dma16(rsrc(abase(c), on ? abytes : 0), b + (wave * XI + j) * 1024, xo[j], c.n * 2);
     } else {
       const int i = j - XI, rows = min(kBN_, N - c.n);
-      dma16(rsrc(wbase(c), on ? rows * K : 0), b + kW + (wave * WI + i) * 1024, wr[i] < rows ? wo[i] : kOOB, 0);
+      dma16(rsrc(wbase(c), on ? rows * ldw : 0), b + kW + (wave * WI + i) * 1024, wr[i] < rows ? wo[i] : kOOB, 0);
     }
   };
   // L2 prefetch: waves 0-3 the rows of a, 64 a wave; waves 4, 5 the two lines of the rows of w
   const int h = min(4, mtiles - at.mt / 4 * 4);
   const bool pw = wave >= 4;
   const int pr = (wave & 3) * 64 + lane, pc = (wave & 3) * 128;
-  const bool mine = pw ? pc < BN && k0 + pc < K && at.mt % h == (lane & 3) % h
+  const bool mine = pw ? pc < BN && k0 + pc < ldw && at.mt % h == (lane & 3) % h
                        : pr < mrows && (at.nt & 3) == (wave & 3);
-  const uint32_t po = !mine ? kOOB : pw ? (uint32_t)lane * (uint32_t)K + (uint32_t)(k0 + pc) : (uint32_t)(pr * np * 2);
+  const uint32_t po = !mine ? kOOB : pw ? (uint32_t)lane * (uint32_t)ldw + (uint32_t)(k0 + pc) : (uint32_t)(pr * np * 2);
   auto prefetch = [&](const Cursor& c) __attribute__((always_inline)) {
     const bool on = c.st < ns;
     const int rows = min(kBN_, N - c.n);
     if (pw)
-      dma4(rsrc(wbase(c), on ? rows * K : 0), smem + R * kStage + wave * 256, lane < rows ? po : kOOB, 0);
+      dma4(rsrc(wbase(c), on ? rows * ldw : 0), smem + R * kStage + wave * 256, lane < rows ? po : kOOB, 0);
     else
       dma4(rsrc(abase(c), on ? abytes : 0), smem + R * kStage + wave * 256, po, c.n * 2);
   };
@@ -231,8 +231,8 @@ int8_bwd_kernel(Int8BwdParams P) {
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int a = 0; a < NT; ++a)
-        if (mw + 16 * i < M && kw + 16 * a < K)  // K is a multiple of 16
-          *reinterpret_cast<f32x4_t*>(P.part + ((size_t)at.split * M + mw + 16 * i) * K + kw + 16 * a) = acc[a][i];
+        if (mw + 16 * i < M && kw + 16 * a < ldw)
+          *reinterpret_cast<f32x4_t*>(P.part + ((size_t)at.split * M + mw + 16 * i) * ldw + kw + 16 * a) = acc[a][i];
     return;
   }
   float row[MT];
@@ -255,20 +255,23 @@ int8_bwd_kernel(Int8BwdParams P) {
         float v[1][4];
         values(i, a, v);
         if (mw + 16 * i < M && kw + 16 * a < K)
-          store4(P.dx, (int64_t)(mw + 16 * i) * K + kw + 16 * a, P.type, P.vec, 4, v[0]);
+          store4(P.dx, (int64_t)(mw + 16 * i) * K + kw + 16 * a, P.type, P.vec, K - kw - 16 * a, v[0]);
       }
   }
 }
 
 // The ranges' sums, added in their order.
 __global__ void __launch_bounds__(256) int8_bwd_reduce_kernel(Int8BwdParams P) {
-  const int64_t mk4 = (int64_t)P.M * P.K / 4, k4 = P.K / 4;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < mk4; i += (int64_t)gridDim.x * 256) {
+  const int64_t l4 = P.ldw / 4, total = l4 * P.M;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t m = i / l4;
+    const int k = (int)(i - m * l4) * 4;
+    if (k >= P.K) continue;
     const f32x4_t* p = reinterpret_cast<const f32x4_t*>(P.part) + i;
-    const f32x4_t v = add_splits<8>(p[0], p, mk4, 1, P.ks);
-    const float row = P.row[i / k4];
+    const f32x4_t v = add_splits<8>(p[0], p, total, 1, P.ks);
+    const float row = P.row[m];
     const float o[4] = {v[0] * row, v[1] * row, v[2] * row, v[3] * row};
-    store4(P.dx, 4 * i, P.type, P.vec, 4, o);
+    store4(P.dx, m * P.K + k, P.type, P.vec, P.K - k, o);
   }
 }
 
@@ -295,11 +298,6 @@ hipError_t launch_tile(const Int8BwdParams& P, hipStream_t s) {
 }
 
 }  // namespace
-
-// Rows of codes on 16 bytes.
-bool int8_bwd_supported(int64_t K, const void* w, const void* w2) {
-  return ((uintptr_t)w | (uintptr_t)w2 | (uintptr_t)K) % 16 == 0;
-}
 
 // As int8_gemm_plan. Measured, us with the gradient's own pass, 256x256 / 128x256 / 128x128 / 64x128 tiles:
 //   dx [M,4096], sum of 4096   128 rows 31 / 31 / 26 / 25   512 44 / 39 / 41 / 46    2048  87 /  81 /  91 / 126
@@ -343,7 +341,7 @@ hipError_t launch_int8_bwd(const Int8BwdParams& given, hipStream_t s) {
     e = launch_tile<128, 256, 4>(P, s);
   }
   if (e != hipSuccess || P.ks == 1) return e;
-  int64_t g = ((int64_t)P.M * P.K / 4 + 255) / 256;
+  int64_t g = ((int64_t)P.M * P.ldw / 4 + 255) / 256;
   if (g > 8192) g = 8192;
   hipLaunchKernelGGL(int8_bwd_reduce_kernel, dim3((unsigned)g), dim3(256), 0, s, P);
   return hipGetLastError();
