@@ -281,16 +281,5 @@ MI_DEV void store_part(const Int8Params& P, int split, int64_t m, int n, i32x4_t
     }
   }
 }
-template <bool DUAL>
-MI_DEV i32x4_t load_part(const Int8Params& P, int split, int bank, int64_t m, int n) {
-  const int32_t* p = P.part + (((int64_t)split * (DUAL ? 2 : 1) + bank) * P.M + m) * P.N + n;
-  if (P.N % 4 == 0) return *reinterpret_cast<const i32x4_t*>(p);
-  i32x4_t v = {0, 0, 0, 0};
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (n + j < P.N) v[j] = p[j];
-  return v;
-}
-
 }  // namespace i8
 }  // namespace mi

@@ -225,19 +225,29 @@ int8_gemm_kernel(Int8Params P) {
         finish4<DUAL>(P, mw + 16 * i, nw + 16 * a, acc[DUAL ? 2 * a : a][i], acc[DUAL ? 2 * a + 1 : a][i], sx[i], cols[a]);
 }
 
-// The splits' sums, exact in any order, and the scales.
+// The splits' sums, exact in any order, and the scales. (Loads of 8 splits go out before their adds.)
 template <bool DUAL>
 __global__ void __launch_bounds__(256) int8_reduce_kernel(Int8Params P) {
-  const int64_t n4 = ((int64_t)P.N + 3) / 4, total = n4 * P.M;
+  constexpr int B = DUAL ? 2 : 1;
+  const int64_t n4 = ((int64_t)P.N + 3) / 4, total = n4 * P.M, mn = (int64_t)P.M * P.N;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     const int64_t m = i / n4;
     const int n = (int)(i - m * n4) * 4;
-    i32x4_t a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
-    for (int s = 0; s < P.ks; ++s) {
-      a += load_part<DUAL>(P, s, 0, m, n);
-      if constexpr (DUAL) b += load_part<DUAL>(P, s, 1, m, n);
+    const float sx = P.sx[m];
+    const Cols cols = load_cols<DUAL>(P, n);
+    i32x4_t v[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      const int32_t* p = P.part + b * mn + m * P.N + n;
+      if (P.N % 4 == 0) {
+        v[b] = add_splits<8>(v[b], reinterpret_cast<const i32x4_t*>(p), B * mn / 4, 0, P.ks);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < P.N) v[b][j] = add_splits<8>((int32_t)0, p + j, B * mn, 0, P.ks);
+      }
     }
-    finish4<DUAL>(P, m, n, a, b, P.sx[m], load_cols<DUAL>(P, n));
+    finish4<DUAL>(P, m, n, v[0], v[1], sx, cols);
   }
 }
 

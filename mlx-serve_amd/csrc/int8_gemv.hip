@@ -10,6 +10,8 @@
 //
 // One float token (FUSE): each block quantizes it by itself, into LDS, while its first weights are on
 // their way: it is a few KB, and a launch of its own costs more.
+#include <cmath>
+
 #include "int8_stage.h"
 
 namespace mi {
@@ -223,7 +225,9 @@ hipError_t launch_rows(const Int8Params& P, hipStream_t s) {
 double int8_gemv_plan(Int8Params& P) {
   P.nt = P.banks == 1 && P.M > 8 && P.M <= 64 && P.N >= 32 * 256 ? 2 : 1;
   const double blocks = (double)((P.N + 16 * P.nt - 1) / (16 * P.nt));
-  return 3.0 + std::max(1.0, blocks / 256) * (16.0 * P.nt * P.banks + P.M) * P.K / 25e3;
+  // (above 64 rows of two banks the waves' sums fill the LDS of a CU: whole rounds)
+  const double rounds = P.M > 64 && P.banks == 2 ? std::ceil(blocks / 256) : std::max(1.0, blocks / 256);
+  return 3.0 + rounds * (16.0 * P.nt * P.banks + P.M) * P.K / 25e3;
 }
 
 // One token of floats quantized in the launch: four 16-byte vectors a thread. Sizes alone decide, as

@@ -136,9 +136,11 @@ hipError_t launch_type(int8_t* q, float* s, const void* x, int64_t rows, int64_t
   const int64_t nv = K / E;
   if (nv <= 64 && rows > 256) return launch_rows<T, 1, 1>(q, s, x, rows, K, ldq, st);
   if (nv <= 256) return launch_rows<T, 4, 1>(q, s, x, rows, K, ldq, st);
+  // Waves a row, measured: 8192 rows of 14336 bf16 values 72 us with 4, 68 with 8 or 16; 8192 rows of 4096
+  // 25 us with 1 or 8, 20 with 4.
   if (nv <= 512 && rows > 256) return launch_rows<T, 4, 2>(q, s, x, rows, K, ldq, st);
-  if (nv <= 1024 && rows > 256) return launch_rows<T, 4, 4>(q, s, x, rows, K, ldq, st);
-  if (nv <= 2048 && rows > 256) return launch_rows<T, 4, 8>(q, s, x, rows, K, ldq, st);
+  if (nv <= 1024 && rows > 256) return launch_rows<T, 8, 2>(q, s, x, rows, K, ldq, st);
+  if (nv <= 2048 && rows > 256) return launch_rows<T, 8, 4>(q, s, x, rows, K, ldq, st);
   if (nv <= 1024) return launch_rows<T, 16, 1>(q, s, x, rows, K, ldq, st);
   if (nv <= 2048) return launch_rows<T, 16, 2>(q, s, x, rows, K, ldq, st);
   if (nv <= 4096) return launch_rows<T, 16, 4>(q, s, x, rows, K, ldq, st);

@@ -406,28 +406,35 @@ def gather_qmv_down_reduce(act, wd, sd, bd, inds, scores, group_size=None, bits=
 _I8 = {torch.bfloat16: DT_BFLOAT16, torch.float16: DT_FLOAT16, torch.float32: DT_FLOAT32}
 
 
+def _bad(msg):
+    raise MiError(MI_ERR_INVALID, msg)
+
+
 def _i8_type(dtype, what):
     code = _I8.get(dtype)
     if code is None:
-        raise MiError(MI_ERR_INVALID, f"{what} dtype {dtype} not supported (bfloat16, float16, float32)")
+        _bad(f"{what} dtype {dtype} not supported (bfloat16, float16, float32)")
     return code
 
 
 def _i8_linear(N, K, dev, *banks):
     """Every bank is int8 [N, K] with fp32 scales [N], on the device of the activations."""
     for w, s in banks:
-        _contig(w, s)
-        _require(w.dtype == torch.int8, "weights must be int8 [N, K]")
-        _require(tuple(w.shape) == (N, K), f"weights {tuple(w.shape)} do not match [{N}, {K}]")
-        _require(s.dtype == torch.float32 and s.numel() == N, "channel scales must be float32 [N]")
-        _require(w.device == dev and s.device == dev, "tensors on different devices")
+        if not (w.is_contiguous() and s.is_contiguous()):
+            _bad("tensors must be row-contiguous")
+        if w.device != dev or s.device != dev:
+            _bad("tensors on different devices")
+        if w.dtype != torch.int8 or w.shape != (N, K):
+            _bad(f"weights must be int8 [{N}, {K}], got {w.dtype} {tuple(w.shape)}")
+        if s.dtype != torch.float32 or s.numel() != N:
+            _bad("channel scales must be float32 [N]")
 
 
 def _i8_call(fn, dev, need, *args):
     """One library call on dev's current stream, with a workspace from torch's allocator: calls on
     other streams and graphs captured from them have others. need None: a call without one."""
     at = dev.index
-    if at != torch.cuda.current_device():
+    if at != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
             return _i8_call(fn, dev, need, *args)
     # (the raw handle: building a Stream object costs as much as a launch)
@@ -453,10 +460,11 @@ def int8_quantize(x):
     For the tokens of an activation and for the output channels of a weight [N, K]."""
     _contig(x)
     shape, dev = x.shape, x.device
-    _require(len(shape) >= 1 and shape[-1] > 0, "x must be [..., K] with K > 0")
+    if not shape or not shape[-1]:
+        _bad("x must be [..., K] with K > 0")
     code = _i8_type(x.dtype, "x")
     K = shape[-1]
-    q = torch.empty(shape, dtype=torch.int8, device=dev)
+    q = torch.empty_like(x, dtype=torch.int8)
     s = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
     _i8_call(lib().mi_int8_quantize, dev, None, q.data_ptr(), s.data_ptr(), x.data_ptr(), x.numel() // K, K,
              code)
@@ -466,23 +474,28 @@ def int8_quantize(x):
 def _i8_activations(x, x_scales, dtype, K):
     """(x's code, y's dtype) of a forward call."""
     _contig(x, x_scales)
-    _require(x.dim() >= 1 and x.shape[-1] == K, f"x {tuple(x.shape)} must end in K={K}")
+    if x.dim() < 1 or x.shape[-1] != K:
+        _bad(f"x {tuple(x.shape)} must end in K={K}")
     xd = x.dtype
-    if xd == torch.int8:
-        _require(x_scales is not None, "int8 x needs x_scales")
-        _require(x_scales.dtype == torch.float32 and x_scales.numel() * K == x.numel(),
-                 "x_scales must be float32, one a row of x")
-        _require(x_scales.device == x.device, "tensors on different devices")
-        return DT_INT8, torch.bfloat16 if dtype is None else dtype
-    _require(x_scales is None, "x_scales belong to int8 x")
-    return _i8_type(xd, "x"), xd if dtype is None else dtype
+    if xd != torch.int8:
+        if x_scales is not None:
+            _bad("x_scales belong to int8 x")
+        return _i8_type(xd, "x"), xd if dtype is None else dtype
+    if x_scales is None:
+        _bad("int8 x needs x_scales")
+    if x_scales.dtype != torch.float32 or x_scales.numel() * K != x.numel():
+        _bad("x_scales must be float32, one a row of x")
+    if x_scales.device != x.device:
+        _bad("tensors on different devices")
+    return DT_INT8, torch.bfloat16 if dtype is None else dtype
 
 
 def int8_matmul(x, w, w_scales, x_scales=None, bias=None, dtype=None):
     """y[..., n] = sum_k x[..., k] w[n, k] on the int8 matrix cores. w int8 [N, K] with w_scales
     [N] (int8_quantize of a weight); x floats, quantized by row within the call, or int8 codes with
     x_scales. y has `dtype` (default: x's, bfloat16 for codes); bias [N] in it, or None."""
-    _require(w.dim() == 2, "weights must be int8 [N, K]")
+    if w.dim() != 2:
+        _bad("weights must be int8 [N, K]")
     N, K = w.shape
     dev = x.device
     xt, dtype = _i8_activations(x, x_scales, dtype, K)
@@ -490,8 +503,8 @@ def int8_matmul(x, w, w_scales, x_scales=None, bias=None, dtype=None):
     yt = _i8_type(dtype, "y")
     if bias is not None:
         _contig(bias)
-        _require(bias.dtype == dtype and bias.numel() == N and bias.device == dev,
-                 "bias must be [N] in y's dtype, on x's device")
+        if bias.dtype != dtype or bias.numel() != N or bias.device != dev:
+            _bad("bias must be [N] in y's dtype, on x's device")
     M = x.numel() // K if K else 0
     y = torch.empty(x.shape[:-1] + (N,), dtype=dtype, device=dev)
     L = lib()
@@ -503,7 +516,8 @@ def int8_matmul(x, w, w_scales, x_scales=None, bias=None, dtype=None):
 def int8_gate_up_swiglu(x, wg, sg, wu, su, x_scales=None, dtype=None, save=False):
     """silu(x @ wg.T) * (x @ wu.T) in one launch, operands as int8_matmul. save=True returns
     (y, gate, up), the two projections for int8_gate_up_swiglu_backward."""
-    _require(wg.dim() == 2, "weights must be int8 [N, K]")
+    if wg.dim() != 2:
+        _bad("weights must be int8 [N, K]")
     N, K = wg.shape
     dev = x.device
     xt, dtype = _i8_activations(x, x_scales, dtype, K)
@@ -512,8 +526,7 @@ def int8_gate_up_swiglu(x, wg, sg, wu, su, x_scales=None, dtype=None, save=False
     M = x.numel() // K if K else 0
     shape = x.shape[:-1] + (N,)
     y = torch.empty(shape, dtype=dtype, device=dev)
-    gate = torch.empty(shape, dtype=dtype, device=dev) if save else None
-    up = torch.empty(shape, dtype=dtype, device=dev) if save else None
+    gate, up = (torch.empty_like(y), torch.empty_like(y)) if save else (None, None)
     L = lib()
     _i8_call(L.mi_int8_gate_up_swiglu, dev, L.mi_int8_forward_workspace(M, N, K, 2, xt), y.data_ptr(), _at(gate),
              _at(up), x.data_ptr(), _at(x_scales), wg.data_ptr(), sg.data_ptr(), wu.data_ptr(), su.data_ptr(),
@@ -525,10 +538,12 @@ def int8_matmul_backward(dy, w, w_scales):
     """The gradient of int8_matmul to x: dx = (dy * w_scales) @ w, dy [..., N] -> [..., K] (weights
     constant, the rounding of x passed straight through)."""
     _contig(dy)
-    _require(w.dim() == 2, "weights must be int8 [N, K]")
+    if w.dim() != 2:
+        _bad("weights must be int8 [N, K]")
     N, K = w.shape
     dev = dy.device
-    _require(dy.dim() >= 1 and dy.shape[-1] == N, f"dy {tuple(dy.shape)} must end in N={N}")
+    if dy.dim() < 1 or dy.shape[-1] != N:
+        _bad(f"dy {tuple(dy.shape)} must end in N={N}")
     _i8_linear(N, K, dev, (w, w_scales))
     code = _i8_type(dy.dtype, "dy")
     M = dy.numel() // N if N else 0
@@ -542,13 +557,15 @@ def int8_matmul_backward(dy, w, w_scales):
 def int8_gate_up_swiglu_backward(dy, gate, up, wg, sg, wu, su):
     """The gradients of int8_gate_up_swiglu(save=True): (dx [..., K], dgate, dup [..., N])."""
     _contig(dy, gate, up)
-    _require(wg.dim() == 2, "weights must be int8 [N, K]")
+    if wg.dim() != 2:
+        _bad("weights must be int8 [N, K]")
     N, K = wg.shape
     dev = dy.device
-    _require(dy.dim() >= 1 and dy.shape[-1] == N, f"dy {tuple(dy.shape)} must end in N={N}")
-    for t, what in ((gate, "gate"), (up, "up")):
-        _require(t.shape == dy.shape and t.dtype == dy.dtype and t.device == dev,
-                 f"{what} must match dy in shape, dtype and device")
+    if dy.dim() < 1 or dy.shape[-1] != N:
+        _bad(f"dy {tuple(dy.shape)} must end in N={N}")
+    for t in (gate, up):
+        if t.shape != dy.shape or t.dtype != dy.dtype or t.device != dev:
+            _bad("gate and up must match dy in shape, dtype and device")
     _i8_linear(N, K, dev, (wg, sg), (wu, su))
     code = _i8_type(dy.dtype, "dy")
     M = dy.numel() // N if N else 0
