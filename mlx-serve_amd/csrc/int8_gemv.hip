@@ -10,6 +10,8 @@
 //
 // One float token (FUSE): each block quantizes it by itself, into LDS, while its first weights are on
 // their way: it is a few KB, and a launch of its own costs more.
+#include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "int8_stage.h"
@@ -185,6 +187,18 @@ hipError_t launch(const Int8Params& P, hipStream_t s) {
   constexpr int B = DUAL ? 2 : 1;
   size_t lds = (size_t)WK * B * NT * MT * 1024;
   if (XV) lds = std::max(lds, (size_t)256 + (P.K + 63) / 64 * 64);
+  if constexpr (WK * B * NT * MT > 64) {  // past 64 KB (the most is 128 KB: 128 rows of two banks)
+    static std::atomic<uint64_t> done{0};  // devices whose function has the attribute
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    const uint64_t bit = (uint64_t)1 << (dev & 63);
+    if (e == hipSuccess && !(done.load() & bit)) {
+      e = hipFuncSetAttribute((const void*)int8_gemv_kernel<DUAL, MT, NT, WK, U, XV>,
+                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+      if (e == hipSuccess) done |= bit;
+    }
+    if (e != hipSuccess) return e;
+  }
   hipLaunchKernelGGL((int8_gemv_kernel<DUAL, MT, NT, WK, U, XV>),
                      dim3((unsigned)((P.N + 16 * NT - 1) / (16 * NT))), dim3(WK * 64), lds, s, P);
   return hipGetLastError();
