@@ -34,7 +34,7 @@ enum {
   MI_ERR_UNSUPPORTED = 1, /* decline: valid request outside this library's scope */
   MI_ERR_INVALID = 2,     /* bad pointer / shape / argument */
   MI_ERR_HIP = 3,         /* HIP runtime error (launch, allocation) */
-  MI_ERR_WORKSPACE = 4,   /* workspace must grow but the stream is capturing */
+  MI_ERR_WORKSPACE = 4,   /* workspace must grow but the stream is capturing, or the caller's is too small */
 };
 
 /* Values match mlx_dtype (src/mlx.zig:20-35). */
@@ -292,7 +292,8 @@ int mi_gather_qmv_down_reduce(void* y, const void* act, const uint32_t* w_down,
  * this one has run; its size comes from the two functions below (host only; may be 0, then
  * NULL will do; -1 for sizes or types out of range). A missing or short one is
  * MI_ERR_WORKSPACE. These calls allocate nothing and keep nothing, so they can be captured into
- * graphs as they are, and run at the same time on several streams with a workspace each.
+ * graphs as they are, and run at the same time on several streams with a workspace each. Tensors
+ * and stream belong to the current device.
  * Outputs must not overlap inputs. Empty outputs (M = 0, ...) are no-ops; a sum over nothing
  * (K = 0 forward, N = 0 backward) is MI_ERR_INVALID. K over 131071 forward, where the int32 sums
  * of the products could overflow, is MI_ERR_UNSUPPORTED. */

@@ -158,10 +158,9 @@ hipError_t launch_type(int8_t* q, float* s, const void* x, int64_t rows, int64_t
 // Memory-bound (three reads, four writes of [M, N] with both outputs); a row is held in
 // registers between its maximum and the parts.
 
-// power of two for a row whose largest magnitude has these bits, and its reciprocal
+// power of two for a row whose largest finite magnitude has these bits, and its reciprocal
 MI_DEV void row_power(uint32_t maxbits, float* scale, float* inv) {
-  const int e = (int)(maxbits >> 23);
-  const int b = e == 255 || maxbits == 0 ? 127 : min(268 - e, 253);
+  const int b = maxbits == 0 ? 127 : min(268 - (int)(maxbits >> 23), 253);
   *scale = __uint_as_float((uint32_t)b << 23);
   *inv = __uint_as_float((uint32_t)(254 - b) << 23);
 }
@@ -196,7 +195,10 @@ MI_DEV Grad<T> gradient(float dy, float g, float u, float sw, float sw2) {
   }
   return r;
 }
-MI_DEV uint32_t mag(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+MI_DEV uint32_t mag(float v) {  // 0 unless finite
+  const uint32_t m = __float_as_uint(v) & 0x7FFFFFFFu;
+  return m < 0x7F800000u ? m : 0u;
+}
 
 // values of a 16-byte vector
 template <int T, int E>

@@ -115,7 +115,7 @@ def test_matmul_types_and_bias(dev, M, N, K, t):
 
 
 @pytest.mark.parametrize("N,K", [(1, 1), (16, 64), (33, 208), (130, 77), (768, 2048), (2052, 512)])
-@pytest.mark.parametrize("M", [1, 2, 16, 17, 33, 65, 129, 257])
+@pytest.mark.parametrize("M", [1, 2, 16, 17, 33, 65, 100, 128, 129, 257])
 def test_gate_up_sizes(dev, M, N, K):
     _case(t="gate_up", M=M, N=N, K=K)
     g = _gen(M * 7 + N)
@@ -341,6 +341,47 @@ def test_gradients_with_infinite_values(dev, M, t):
     dx = mi_qmm.int8_matmul_backward(bad, w, sw)
     assert torch.equal(dx[1:M - 1], clean[1:M - 1])
     assert torch.isnan(dx[M - 1]).all() and not torch.isfinite(dx[0]).any()
+
+
+@pytest.mark.parametrize("t,big", [(BF16, 1e30), (F16, 3e4), (F32, 1e30)])
+def test_gradients_beside_an_infinity(dev, t, big):
+    """Finite values beside an infinity, larger than fp16 holds, stay finite: the sum is infinite where
+    the infinity's code is not 0, NaN where it is, as the formula has it."""
+    w = torch.tensor([[1, -2, 0, 5], [3, 4, 5, -6], [-7, 8, 9, 10]], dtype=torch.int8, device="cuda").repeat(1, 8)
+    sw = torch.ones(3, device="cuda")
+    dy = torch.tensor([[float("inf"), -big, big], [1.0, big, -big], [2.0 ** -20, 0.0, 1.0]], device="cuda").to(t)
+    dx = mi_qmm.int8_matmul_backward(dy, w, sw)
+    assert torch.isnan(dx[0, 2]) and torch.isinf(dx[0, [0, 1, 3]]).all() and dx[0, 1] < 0 < dx[0, 0]
+    ref, tol = R.matmul_backward(dy[1:], w, sw)
+    # 3e4 (1 * 0 + 3 + 7) is 3e5: past fp16's largest value and half a step (65520) a rounding is infinite
+    ref = torch.where(ref.abs() - tol > torch.finfo(t).max * (1 + torch.finfo(t).eps / 4), ref.sign() * torch.inf, ref)
+    R.check(dx[1:], ref, tol, "finite rows")
+
+
+def test_offsets_past_31_bits(dev):
+    """More than 2^31 values of x and of y: the last rows against the same rows alone."""
+    g = _gen(9)
+    M, K, N = 70001, 31008, 64
+    x = torch.randn(M, K, device="cuda", generator=g, dtype=BF16)
+    q, s = mi_qmm.int8_quantize(x)
+    ql, sl = R.quantize(x[-5:])
+    assert torch.equal(q[-5:], ql) and torch.equal(s[-5:], sl)
+    w, sw = _weights(g, N, K)
+    y = mi_qmm.int8_matmul(q, w, sw, x_scales=s)
+    ref, tol = R.matmul(ql, sl, w, sw)
+    R.check(y[-5:], ref, tol(BF16), "rows far into x")
+    del y, x
+    w, sw = _weights(g, K, N)
+    x = _x(g, M, N, BF16)
+    y = mi_qmm.int8_matmul(x, w, sw)
+    qx, sx = R.quantize(x[-5:])
+    ref, tol = R.matmul(qx, sx, w, sw)
+    R.check(y[-5:], ref, tol(BF16), "rows far into y")
+    dx = mi_qmm.int8_matmul_backward(y, w, sw)
+    R.check(dx[-5:], *R.matmul_backward(y[-5:], w, sw), "rows far into dy")
+    del dx, y
+    dx = mi_qmm.int8_matmul_backward(x, w.t().contiguous(), torch.ones(N, device="cuda"))
+    R.check(dx[-5:], *R.matmul_backward(x[-5:], w.t().contiguous(), torch.ones(N, device="cuda")), "rows far into dx")
 
 
 # ------------------------------------------------- as they are used, and around --
