@@ -12,14 +12,20 @@
 // and stage t + 1 has landed. Vector memory operations return in order, so "landed" is an
 // exact vmcnt.
 //
-// What bounds it: the DMA. Without it the same loop runs 8192 x 4096 x 14336 in 321 us, alone it
-// takes 389 us, together 414: the 64 KB of a step come late when their lines come from HBM or
-// the memory-side cache. So each block asks the L2 for its lines two steps before it moves them
-// (one dword a line, into a corner of LDS that nothing reads), and the blocks of a panel that
-// share a tile of x or w (prefill_tiles.h) each ask for a part of it: alone 292 us, together 398
-// (2.4 POPS; 420 in a row at the clock that the card's power allows then).
-// Against 64-byte steps in a ring of five stages (444 us) and weights straight into registers
-// (455 us).
+// What bounds it: large products the matrix cores and the DMA beside them at the clock that the card's
+// power allows: 8192 x 4096 x 14336 in 361 us, 2.66 POPS (a library product of the same codes: 402 to
+// 459 us, by their values); MFMA instructions are busy 67% of the time. 64-byte steps in a ring of
+// five stages took 444 us, weights straight into registers 455. Up to 256 rows or so the weights
+// from HBM bound it: gate + up [14336,4096], 48 rows, 25.9 us (4.5 TB/s). Two things keep them coming:
+// - Rows of a power-of-two pitch meet in the same memory channels. Up to 256 rows a column tile starts
+//   3 steps further along K than the one before it and wraps round (int32 sums, exact in any
+//   order): 25.9 us against 30.6 there. With more rows tiles share lines in the L2 by reading them
+//   at the same time, and it costs up to 2%.
+// - A ring of two stages is short for weights from HBM: where all blocks run in one round (AHEAD), each
+//   asks the L2 for its lines two steps before it moves them (one dword a line, into a corner of
+//   LDS that nothing reads; the blocks of a panel that share a tile of x or w, prefill_tiles.h,
+//   each for a part): gate + up 512 rows 59 us against 65, 128 rows 35 against 40. With more rounds
+//   (8192 rows 361 / 371) and with three stages (25.9 / 31) it costs time: a line then comes in parts.
 //
 // K: any multiple of 16. In the last step the slots from K on load out of bounds, as zeros.
 #include <algorithm>
@@ -34,6 +40,7 @@ namespace {
 
 using namespace i8;
 constexpr int kBK = 128;
+constexpr int kStagger = 3;  // steps; 2, 5, 8, 11 and 13 are within 2% of it, 16 (2 KB) is 45% slower
 
 template <int BM, int BN, int R>
 constexpr int lds_bytes() { return R * (BM + BN) * kBK + 2048; }
@@ -41,7 +48,7 @@ constexpr int lds_bytes() { return R * (BM + BN) * kBK + 2048; }
 // waves a SIMD: 2 (one block a CU), 4 for the small tiles (two blocks, whose starts and ends overlap)
 constexpr int eu_waves(int bm, int bn) { return bm * bn <= 128 * 128 ? 4 : 2; }
 
-template <bool DUAL, int BM, int BN, int R, bool SPLIT>
+template <bool DUAL, int BM, int BN, int R, bool SPLIT, bool AHEAD>
 __global__ void __launch_bounds__(512)
     __attribute__((amdgpu_waves_per_eu(eu_waves(BM, BN), eu_waves(BM, BN))))
 int8_gemm_kernel(Int8Params P) {
@@ -71,19 +78,23 @@ int8_gemm_kernel(Int8Params P) {
   for (int i = 0; i < XI; ++i) {
     const int r = 8 * (wave * XI + i) + (lane >> 3);
     xc[i] = 16 * ((lane & 7) ^ xswz(r));
-    xo[i] = (uint32_t)(min(r, mrows - 1) * ldx + xc[i]);
+    xo[i] = r < mrows ? (uint32_t)(r * ldx + xc[i]) : kOOB;
   }
 #pragma unroll
   for (int i = 0; i < WI; ++i) {
     const int r = 8 * (wave * WI + i) + (lane >> 3);
     const int row = DUAL ? 16 * (r >> 5) + (r & 15) : r;  // tiles alternate gate, up
     wc[i] = 16 * ((lane & 7) ^ xswz(r));
-    wo[i] = (uint32_t)min(row, nrows - 1) * (uint32_t)K + wc[i];
+    wo[i] = row < nrows ? (uint32_t)row * (uint32_t)K + wc[i] : kOOB;
   }
   // stages past the range load through a resource of zero records (zeros, no traffic)
+  const int first = M <= 256 ? at.nt * kStagger % ns : 0;
+  auto place = [&](int st) __attribute__((always_inline)) {  // of step st along K
+    return (s0 + st + (st + first < ns ? first : first - ns)) * kBK;
+  };
   auto issue = [&](int st, int slot) __attribute__((always_inline)) {
     const bool on = st < ns;
-    const int k = (s0 + st) * kBK;
+    const int k = place(st);
     unsigned char* b = smem + slot * kStage;
 #pragma unroll
     for (int i = 0; i < XI; ++i)
@@ -95,6 +106,7 @@ int8_gemm_kernel(Int8Params P) {
   };
   // L2 prefetch: waves 0-3 the rows of x, 4-7 those of w (4, 5 gate and 6, 7 up), 64 a wave. The h
   // blocks of a panel that read this w tile split its rows, four of those that read x its.
+  constexpr int PF = AHEAD ? 1 : 0;  // instructions a step
   const int h = min(4, mtiles - at.mt / 4 * 4);
   const bool pw = wave >= 4;
   const int8_t* pb = !pw ? xb : DUAL && (wave & 2) ? wb2 : wb;
@@ -102,7 +114,8 @@ int8_gemm_kernel(Int8Params P) {
   const bool mine = pr < pn && (pw ? at.mt % h == (wave & 3) % h : (at.nt & 3) == (wave & 3));
   const uint32_t po = mine ? (uint32_t)pr * (uint32_t)(pw ? K : ldx) : kOOB;
   auto prefetch = [&](int st) __attribute__((always_inline)) {
-    dma4(rsrc(pb, st < ns ? (pw ? wbytes : xbytes) : 0), smem + R * kStage + wave * 256, po, (s0 + st) * kBK);
+    if constexpr (PF)
+      dma4(rsrc(pb, st < ns ? (pw ? wbytes : xbytes) : 0), smem + R * kStage + wave * 256, po, place(st));
   };
 
   i32x4_t acc[NT][MT];
@@ -134,7 +147,7 @@ int8_gemm_kernel(Int8Params P) {
     prefetch(s + R);
     __builtin_amdgcn_sched_barrier(0);
   }
-  wait_vm(1 + (R - 1) * (XI + WI + 1));
+  wait_vm(PF + (R - 1) * (XI + WI + PF));
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_sched_barrier(0);
   frags(0, 0);
@@ -152,7 +165,7 @@ int8_gemm_kernel(Int8Params P) {
     }
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): this wave's reads of stage t
-    wait_vm(1 + (R - 2) * (XI + WI + 1));
+    wait_vm(PF + (R - 2) * (XI + WI + PF));
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
     frags(next, 0);
@@ -251,26 +264,34 @@ __global__ void __launch_bounds__(256) int8_reduce_kernel(Int8Params P) {
   }
 }
 
-template <bool DUAL, int BM, int BN, int R>
-hipError_t launch_tile(const Int8Params& P, hipStream_t s) {
+template <bool DUAL, int BM, int BN, int R, bool SPLIT, bool AHEAD>
+hipError_t launch_kernel(const Int8Params& P, dim3 grid, hipStream_t s) {
   constexpr int lds = lds_bytes<BM, BN, R>();
-  static std::atomic<uint64_t> done{0};  // devices whose functions have the attribute
+  const auto kernel = int8_gemm_kernel<DUAL, BM, BN, R, SPLIT, AHEAD>;
+  static std::atomic<uint64_t> done{0};  // devices whose function has the attribute
   int dev = 0;
   hipError_t e = hipGetDevice(&dev);
   const uint64_t bit = (uint64_t)1 << (dev & 63);
   if (e == hipSuccess && !(done.load() & bit)) {
-    for (auto k : {int8_gemm_kernel<DUAL, BM, BN, R, false>, int8_gemm_kernel<DUAL, BM, BN, R, true>})
-      if (e == hipSuccess)
-        e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e == hipSuccess) done |= bit;
   }
   if (e != hipSuccess) return e;
-  const dim3 grid((unsigned)(((P.M + BM - 1) / BM) * (P.ct1 - P.ct0)), (unsigned)P.ks);
-  if (P.ks > 1)
-    hipLaunchKernelGGL((int8_gemm_kernel<DUAL, BM, BN, R, true>), grid, dim3(512), lds, s, P);
-  else
-    hipLaunchKernelGGL((int8_gemm_kernel<DUAL, BM, BN, R, false>), grid, dim3(512), lds, s, P);
+  hipLaunchKernelGGL(kernel, grid, dim3(512), lds, s, P);
   return hipGetLastError();
+}
+
+template <bool DUAL, int BM, int BN, int R>
+hipError_t launch_tile(const Int8Params& P, hipStream_t s) {
+  const dim3 grid((unsigned)(((P.M + BM - 1) / BM) * (P.ct1 - P.ct0)), (unsigned)P.ks);
+  const bool split = P.ks > 1;
+  if constexpr (R == 2) {
+    if ((uint64_t)grid.x * grid.y <= 256)
+      return split ? launch_kernel<DUAL, BM, BN, R, true, true>(P, grid, s)
+                   : launch_kernel<DUAL, BM, BN, R, false, true>(P, grid, s);
+  }
+  return split ? launch_kernel<DUAL, BM, BN, R, true, false>(P, grid, s)
+               : launch_kernel<DUAL, BM, BN, R, false, false>(P, grid, s);
 }
 
 template <bool DUAL>
@@ -300,14 +321,14 @@ hipError_t launch_gemm(Int8Params P, hipStream_t s) {
 // partials written and read back with the reduce launch, and the time that the operands take
 // from HBM at least. Depends on the sizes alone (not on pointers), so the workspace can be asked
 // for ahead. Measured, us, with 256x256 / 128x256 / 128x128 / 64x128 tiles:
-//   [14336,4096]  128 rows 35 / 33 / 29 / 27   512 57 / 41 / 47 / 61   2048 128 / 154 / 153 / 199
-//   [4096,4096]   128 rows 25 / 24 / 20 / 17   512 34 / 28 / 26 / 21   2048  55 /  40 /  45 /  61
-//   [4096,14336]  128 rows 34 / 31 / 28 / 29   512 54 / 48 / 57 / 63   2048 124 / 117 / 140 / 193
-//   gate + up [14336,4096] 256 rows 61 / 43 / 50 / 62, 1024 120 / 141 / 153 / 194
+//   [14336,4096]  128 rows 33 / 28 / 29 / 22   512 55 / 39 / 44 / 56   2048 119 / 145 / 151 / 183
+//   [4096,4096]   128 rows 21 / 23 / 19 / 17   512 33 / 26 / 25 / 19   2048  51 /  40 /  41 /  56
+//   [4096,14336]  128 rows 34 / 29 / 28 / 27   512 53 / 45 / 54 / 61   2048 124 / 116 / 130 / 175
+//   gate + up [14336,4096] 256 rows 60 / 42 / 47 / 60, 1024 122 / 141 / 156 / 183
 double int8_gemm_plan(Int8Params& P) {
   const int steps = (P.K + kBK - 1) / kBK, banks = P.banks;
   constexpr TileCost kTiles[] = {
-      {256, 256, 1.72, 0.0, 8.0}, {128, 256, 1.03, 0.0, 4.0}, {128, 128, 0.75, 1.13, 3.0}, {64, 128, 0.55, 0.8, 3.0}};
+      {256, 256, 1.55, 0.0, 8.0}, {128, 256, 1.03, 0.0, 4.0}, {128, 128, 0.75, 1.13, 3.0}, {64, 128, 0.5, 0.8, 2.5}};
   double best = 1e30;
   for (const TileCost& t : kTiles) {
     const int on = t.bn / banks;
@@ -327,7 +348,7 @@ double int8_gemm_plan(Int8Params& P) {
       }
     }
   }
-  return 3.0 + std::max(best, ((double)banks * P.N + P.M) * P.K / 4.4e6);
+  return 3.0 + std::max(best, ((double)banks * P.N + P.M) * P.K / 5e6);
 }
 
 hipError_t launch_int8_gemm(const Int8Params& P, hipStream_t s) {

@@ -9,7 +9,14 @@
 // by the second bank), which is why wide calls take two tiles a wave.
 //
 // One float token (FUSE): each block quantizes it by itself, into LDS, while its first weights are on
-// their way: it is a few KB, and a launch of its own costs more.
+// their way: it is a few KB, and a launch of its own costs more (2 us and the gap before it).
+//
+// Measured in graphs, us: [14336,4096] 1 token 15.7, 2 rows 14.6 (4.0 TB/s), 8 rows 17.0;
+// [4096,14336] 14.5, 13.4 and 15.7; [4096,4096] 6.2, 5.9 and 6.4; gate + up [14336,4096] 1 token 27.5
+// (4.3 TB/s), 16 rows 29. Above 16 rows the reads of x from the L2 count: [4096,4096] 16 rows 7.4,
+// 64 rows 13.2. (Two chunks that share a line, 16 of each 32 bytes for either, so that the first load
+// asks for the whole line, took 0.2 us off one token of [4096,4096] and put up to 1.3 us on 8 rows;
+// starts of the blocks along K moved apart, as in int8_gemm.hip, cost 10 to 20%.)
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -232,16 +239,17 @@ hipError_t launch_rows(const Int8Params& P, hipStream_t s) {
 
 }  // namespace
 
-// Tiles of a wave, and the estimated microseconds: a CU takes about 25 KB of weights and x in a
-// microsecond, over rounds of 256 blocks. Two tiles (one bank) halve what is read of x, where
-// they leave a block for each CU. Measured, one / two tiles a wave: [14336,4096] 2 rows 14.7 /
-// 16.0 us, 16 rows 20.9 / 17.5; [4096,14336] 16 rows 20.1 / 23.7.
+// Tiles of a wave, and the estimated microseconds: a CU takes about 32 KB of weights and x in a
+// microsecond, over rounds of 256 blocks, and the weights come at 3.6 TB/s at most. Two tiles (one
+// bank) halve what is read of x, where they leave a block for each CU. Measured, one / two tiles a
+// wave: [14336,4096] 2 rows 14.7 / 16.0 us, 16 rows 20.9 / 17.5; [4096,14336] 16 rows 20.1 / 23.7.
+// Against int8_gemm.hip, here / there, 16, 32, 64 and 128 rows: [4096,4096] 7.4 / 10.8, 8.6 / 11.9,
+// 13.2 / 15.0, 20.5 / 16.1; [4096,14336] 20.2 / 18.8, 25 / 18.2, 40 / 19.6, 66 / 25.1; gate + up [5632,2048]
+// 8.9 / 13.5, 11.2 / 11.8, 15.5 / 12.4, 25.0 / 12.2.
 double int8_gemv_plan(Int8Params& P) {
   P.nt = P.banks == 1 && P.M > 8 && P.M <= 64 && P.N >= 32 * 256 ? 2 : 1;
-  const double blocks = (double)((P.N + 16 * P.nt - 1) / (16 * P.nt));
-  // (above 64 rows of two banks the waves' sums fill the LDS of a CU: whole rounds)
-  const double rounds = P.M > 64 && P.banks == 2 ? std::ceil(blocks / 256) : std::max(1.0, blocks / 256);
-  return 3.0 + rounds * (16.0 * P.nt * P.banks + P.M) * P.K / 25e3;
+  const double rounds = std::ceil((double)((P.N + 16 * P.nt - 1) / (16 * P.nt)) / 256);
+  return 3.5 + std::max(rounds * (16.0 * P.nt * P.banks + P.M) * P.K / 32e3, (double)P.banks * P.N * P.K / 3.6e6);
 }
 
 // One token of floats quantized in the launch: four 16-byte vectors a thread. Sizes alone decide, as
