@@ -6,11 +6,18 @@
 // Block: 8 waves as 2 (rows of a) x 4 (columns of w), BM x BN outputs, v_mfma_f32_16x16x32_f16 with
 // D[k][m] = w[n][k] a[m][n]. A step is 64 values of n: rows of a are one cache line, the codes 64
 // rows of BN bytes, both moved by LDS DMA into a ring of R stages as in int8_gemm.hip (one barrier a
-// step, in its middle; the L2 asked for lines ahead). The sum runs along the rows of w, so a
+// step, in its middle). The sum runs along the rows of w, so a
 // fragment takes one column of eight rows: ds_read_b64_tr_b8 gives lane l of 16 column l % 16 of the
 // 8 x 16 bytes that the 16 lanes point at, so w is read as it lies in memory, and no turned copy of
 // it is made. Codes become fp16 in registers, five operations for four: u = code + 128 in the low
 // byte of 0x64 is 1024 + u, minus 1152.
+//
+// What bounds it: the matrix cores at the clock that the card's power allows. dx [4096,4096] of gate
+// + up [14336,4096] takes 660 to 690 us behind the gradient's pass, 1.4 to 1.45 PFLOP/s, where a bf16
+// library product of 8192^3 runs at 1.41; MFMA instructions are busy 78% of the time. Without an alias
+// scope of the turned reads (read_tr8) it took 90 us more, stored straight from the products' layout
+// 13 us more. A dword of each line asked for in the L2 ahead of the DMA, which helps short rings in
+// int8_gemm.hip, made it 2 to 8% slower at every size and tile.
 #include <algorithm>
 #include <atomic>
 
@@ -26,7 +33,7 @@ constexpr int kBN_ = 64;  // values of n a step
 typedef int32_t i32x2_t __attribute__((ext_vector_type(2)));
 
 template <int BM, int BN, int R>
-constexpr int lds_bytes() { return R * (BM * 128 + kBN_ * BN) + 2048; }
+constexpr int lds_bytes() { return R * (BM * 128 + kBN_ * BN); }
 
 // Swizzle of the 16-byte slots of a row of codes. A pass of 32 lanes reads one slot of 16 rows:
 // rows 8e .. 8e+7 of quarters q and q + 1 (n = 16 q + 8 e + j): j and the parity of q tell them
@@ -119,22 +126,6 @@ int8_bwd_kernel(Int8BwdParams P) {
       dma16(rsrc(wbase(c), on ? rows * ldw : 0), b + kW + (wave * WI + i) * 1024, wr[i] < rows ? wo[i] : kOOB, 0);
     }
   };
-  // L2 prefetch: waves 0-3 the rows of a, 64 a wave; waves 4, 5 the two lines of the rows of w
-  const int h = min(4, mtiles - at.mt / 4 * 4);
-  const bool pw = wave >= 4;
-  const int pr = (wave & 3) * 64 + lane, pc = (wave & 3) * 128;
-  const bool mine = pw ? pc < BN && k0 + pc < ldw && at.mt % h == (lane & 3) % h
-                       : pr < mrows && (at.nt & 3) == (wave & 3);
-  const uint32_t po = !mine ? kOOB : pw ? (uint32_t)lane * (uint32_t)ldw + (uint32_t)(k0 + pc) : (uint32_t)(pr * np * 2);
-  auto prefetch = [&](const Cursor& c) __attribute__((always_inline)) {
-    const bool on = c.st < ns;
-    const int rows = min(kBN_, N - c.n);
-    if (pw)
-      dma4(rsrc(wbase(c), on ? rows * ldw : 0), smem + R * kStage + wave * 256, lane < rows ? po : kOOB, 0);
-    else
-      dma4(rsrc(abase(c), on ? abytes : 0), smem + R * kStage + wave * 256, po, c.n * 2);
-  };
-
   f32x4_t acc[NT][MT];
 #pragma unroll
   for (int a = 0; a < NT; ++a)
@@ -190,17 +181,15 @@ int8_bwd_kernel(Int8BwdParams P) {
   };
   static_assert(NT % 2 == 0, "a half ends on the tile buffer it began on");
 
-  Cursor ci = start(0), cp = start(R);
+  Cursor ci = start(0);
 #pragma unroll
   for (int s = 0; s < R; ++s) {
 #pragma unroll
     for (int j = 0; j < XI + WI; ++j) issue(ci, s, j);
-    prefetch(cp);
     step(ci);
-    step(cp);
     __builtin_amdgcn_sched_barrier(0);
   }
-  wait_vm(1 + (R - 1) * (XI + WI + 1));
+  wait_vm((R - 1) * (XI + WI));
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_sched_barrier(0);
   read_a(0, 0);
@@ -213,13 +202,11 @@ int8_bwd_kernel(Int8BwdParams P) {
     const int next = slot + 1 == R ? 0 : slot + 1;
     half(0, slot, false, ci, slot);
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): this wave's reads of stage t
-    wait_vm(1 + (R - 2) * (XI + WI + 1));
+    wait_vm((R - 2) * (XI + WI));
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
     half(1, next, true, ci, slot);
-    prefetch(cp);
     step(ci);
-    step(cp);
     slot = next;
   }
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // no DMA may outlive the block
@@ -299,14 +286,15 @@ hipError_t launch_tile(const Int8BwdParams& P, hipStream_t s) {
 
 }  // namespace
 
-// As int8_gemm_plan. Measured, us with the gradient's own pass, 256x256 / 128x256 / 128x128 / 64x128 tiles:
-//   dx [M,4096], sum of 4096   128 rows 31 / 31 / 26 / 25   512 44 / 39 / 41 / 46    2048  87 /  81 /  91 / 126
-//   dx [M,14336], sum of 4096  128 rows 46 / 41 / 43 / 47   512 80 / 75 / 84 / 124   2048 219 / 285 / 280 / 410
-//   dx [M,4096], gate + up sums of 14336  77 rows 69 / 61 / 59 / 74    4096 847 / 1078 / 1197 / 1690
+// As int8_gemm_plan. Measured, us with the gradient's own pass, 256x256 / 128x256 / 128x128 tiles:
+//   dx [M,4096], sum of 4096   300 rows 39 / 32 / 33   1024 57 / 54 / 50    2048  85 /  75 /  84
+//   dx [M,14336], sum of 4096  300 rows 73 / 66 / 74   1024 111 / 139 / 150  2048 205 / 260 / 258
+//   dx [M,4096], gate + up sums of 14336   512 rows 142 / 158 / 172   4096 829 / 1016 / 1100
+// and 64x128, which lasts for few rows: dx [128,4096] of 4096 30 / 29 / 25 / 25.
 void int8_bwd_plan(Int8BwdParams& P) {
   const int steps = P.banks * P.terms * (P.np / kBN_);
   constexpr TileCost kTiles[] = {
-      {256, 256, 1.55, 0.0, 8.0}, {128, 256, 1.0, 0.0, 4.0}, {128, 128, 0.75, 1.0, 3.0}, {64, 128, 0.6, 0.84, 3.0}};
+      {256, 256, 1.47, 0.0, 8.0}, {128, 256, 0.92, 0.0, 4.0}, {128, 128, 0.68, 1.07, 3.0}, {64, 128, 0.57, 0.8, 3.0}};
   double best = 1e30;
   for (const TileCost& t : kTiles) {
     const int64_t tiles = (int64_t)((P.M + t.bm - 1) / t.bm) * ((P.K + t.bn - 1) / t.bn);

@@ -219,7 +219,9 @@ def test_unaligned_pointers(dev, M):
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("M,N,K", [(1100, 9000, 2064), (2600, 7700, 2064), (2600, 7701, 1040), (600, 5002, 2064),
                                    (1300, 2000, 1040), (300, 1000, 4112), (600, 1001, 8208), (150, 700, 8208),
-                                   (129, 24, 16400), (257, 4104, 16)])
+                                   (129, 24, 16400), (257, 4104, 16), (129, 24301, 64), (3615, 38, 9232), (3588, 40, 10112),
+                                   (165, 22405, 1296), (141, 4469, 9792), (1784, 16822, 272), (6205, 6142, 608),
+                                   (457, 17435, 12448), (146, 12147, 9600)])
 def test_matmul_tiles(dev, M, N, K, t):
     _case(t="matmul_tiles", M=M, N=N, K=K, type=t)
     g = _gen(M + N)
@@ -235,7 +237,9 @@ def test_matmul_tiles(dev, M, N, K, t):
 
 @pytest.mark.parametrize("t,save", [(BF16, True), (F16, False), (F32, True)])
 @pytest.mark.parametrize("M,N,K", [(1100, 4500, 2064), (1300, 13000, 1040), (600, 2501, 2064), (300, 1000, 4112),
-                                   (600, 1000, 8208), (150, 350, 8208), (700, 10000, 528)])
+                                   (600, 1000, 8208), (150, 350, 8208), (700, 10000, 528), (129, 35, 64), (135, 12137, 64),
+                                   (1673, 257, 8064), (158, 11369, 1184), (139, 3614, 6048), (464, 30050, 272),
+                                   (7836, 1312, 784), (135, 17529, 10144), (136, 5754, 9472)])
 def test_gate_up_tiles(dev, M, N, K, t, save):
     _case(t="gate_up_tiles", M=M, N=N, K=K, type=t)
     g = _gen(M + N)
@@ -252,7 +256,8 @@ def test_gate_up_tiles(dev, M, N, K, t, save):
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("M,K,N", [(520, 32992, 130), (1100, 9008, 2050), (2600, 7696, 1026), (600, 5008, 2050),
                                    (130, 5008, 2050), (300, 1008, 4100), (600, 1008, 8200), (70, 528, 8200),
-                                   (257, 16, 2049)])
+                                   (257, 16, 2049), (204, 32, 8282), (2621, 144, 5040), (3313, 288, 12279),
+                                   (520, 16512, 1030), (3313, 8208, 260)])
 def test_matmul_backward_tiles(dev, M, K, N, t):
     _case(t="matmul_bwd_tiles", M=M, N=N, K=K, type=t)
     g = _gen(M + N)
