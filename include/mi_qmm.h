@@ -290,8 +290,9 @@ int mi_gather_qmv_down_reduce(void* y, const void* act, const uint32_t* w_down,
  *
  * Workspace: device memory of the caller's, aligned to 16 bytes, that no other call uses until
  * this one has run; its size comes from the two functions below (host only; may be 0, then
- * NULL will do; -1 for sizes or types out of range). A missing or short one is
- * MI_ERR_WORKSPACE. These calls allocate nothing and keep nothing, so they can be captured into
+ * NULL will do; -1 for sizes or types out of range). It holds the quantized tokens, scaled gradients
+ * or partial sums, and, where K is no multiple of 16, a copy of the weights in rows that are: lay such
+ * weights out with zeros up to 16 for speed. A missing or short one is MI_ERR_WORKSPACE. These calls allocate nothing and keep nothing, so they can be captured into
  * graphs as they are, and run at the same time on several streams with a workspace each. Tensors
  * and stream belong to the current device.
  * Outputs must not overlap inputs. Empty outputs (M = 0, ...) are no-ops; a sum over nothing

