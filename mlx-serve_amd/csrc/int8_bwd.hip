@@ -294,13 +294,13 @@ hipError_t launch_tile(const Int8BwdParams& P, hipStream_t s) {
 void int8_bwd_plan(Int8BwdParams& P) {
   const int steps = P.banks * P.terms * (P.np / kBN_);
   constexpr TileCost kTiles[] = {
-      {256, 256, 1.47, 0.0, 8.0}, {128, 256, 0.92, 0.0, 4.0}, {128, 128, 0.68, 1.07, 3.0}, {64, 128, 0.57, 0.8, 3.0}};
+      {256, 256, 1.47, 0.0, 8.0}, {128, 256, 0.92, 0.0, 4.0}, {128, 128, 0.6, 1.07, 3.0}, {64, 128, 0.5, 0.8, 3.0}};
   double best = 1e30;
   for (const TileCost& t : kTiles) {
     const int64_t tiles = (int64_t)((P.M + t.bm - 1) / t.bm) * ((P.K + t.bn - 1) / t.bn);
     for (int k = 1; k <= std::max(1, steps / 4) && k <= 64; ++k) {
       const int sps = (steps + k - 1) / k, ks = (steps + sps - 1) / sps;
-      const double part = ks > 1 ? (double)ks * P.M * P.K * 8 / 5e6 + 3.0 : 0.0;
+      const double part = ks > 1 ? (double)ks * P.M * P.K * 8 / 4.2e6 + 3.0 : 0.0;
       double cost = tile_us(t, tiles * ks, sps) + part;
       const int tail = t.bm == 256 && ks == 1 ? tail_columns(t, kTiles[1], P.M, (P.K + 255) / 256, steps, &cost) : 0;
       if (cost < best - 1e-9) {
