@@ -454,6 +454,13 @@ def _at(t):
     return None if t is None else t.data_ptr()
 
 
+def _i8_out(like, M, N, dtype, dev):
+    """[..., N] for the M rows of `like`. (By strides, two numbers each: a torch.Size in a size
+    argument costs a microsecond more.)"""
+    y = torch.empty_strided((M, N), (max(N, 1), 1), dtype=dtype, device=dev)
+    return y if like.dim() == 2 else y.view(like.shape[:-1] + (N,))
+
+
 def int8_quantize(x):
     """Rows of x [..., K] (bfloat16, float16 or float32) -> (int8 codes [..., K], float32 scales
     [...]): scale = max |x| / 127, code = the nearest integer to x / scale, ties to even.
@@ -465,17 +472,17 @@ def int8_quantize(x):
     code = _i8_type(x.dtype, "x")
     K = shape[-1]
     q = torch.empty_like(x, dtype=torch.int8)
-    s = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
-    _i8_call(lib().mi_int8_quantize, dev, None, q.data_ptr(), s.data_ptr(), x.data_ptr(), x.numel() // K, K,
-             code)
-    return q, s
+    rows = x.numel() // K
+    s = torch.empty(rows, dtype=torch.float32, device=dev)
+    _i8_call(lib().mi_int8_quantize, dev, None, q.data_ptr(), s.data_ptr(), x.data_ptr(), rows, K, code)
+    return q, s if len(shape) == 2 else s.view(shape[:-1])
 
 
 def _i8_activations(x, x_scales, dtype, K):
     """(x's code, y's dtype) of a forward call."""
     _contig(x, x_scales)
-    if x.dim() < 1 or x.shape[-1] != K:
-        _bad(f"x {tuple(x.shape)} must end in K={K}")
+    if x.dim() < 1 or x.shape[-1] != K or not K:
+        _bad(f"x {tuple(x.shape)} must end in K={K}, over 0")
     xd = x.dtype
     if xd != torch.int8:
         if x_scales is not None:
@@ -505,8 +512,8 @@ def int8_matmul(x, w, w_scales, x_scales=None, bias=None, dtype=None):
         _contig(bias)
         if bias.dtype != dtype or bias.numel() != N or bias.device != dev:
             _bad("bias must be [N] in y's dtype, on x's device")
-    M = x.numel() // K if K else 0
-    y = torch.empty(x.shape[:-1] + (N,), dtype=dtype, device=dev)
+    M = x.numel() // K
+    y = _i8_out(x, M, N, dtype, dev)
     L = lib()
     _i8_call(L.mi_int8_matmul, dev, L.mi_int8_forward_workspace(M, N, K, 1, xt), y.data_ptr(), x.data_ptr(),
              _at(x_scales), w.data_ptr(), w_scales.data_ptr(), _at(bias), M, N, K, xt, yt)
@@ -523,9 +530,8 @@ def int8_gate_up_swiglu(x, wg, sg, wu, su, x_scales=None, dtype=None, save=False
     xt, dtype = _i8_activations(x, x_scales, dtype, K)
     _i8_linear(N, K, dev, (wg, sg), (wu, su))
     yt = _i8_type(dtype, "y")
-    M = x.numel() // K if K else 0
-    shape = x.shape[:-1] + (N,)
-    y = torch.empty(shape, dtype=dtype, device=dev)
+    M = x.numel() // K
+    y = _i8_out(x, M, N, dtype, dev)
     gate, up = (torch.empty_like(y), torch.empty_like(y)) if save else (None, None)
     L = lib()
     _i8_call(L.mi_int8_gate_up_swiglu, dev, L.mi_int8_forward_workspace(M, N, K, 2, xt), y.data_ptr(), _at(gate),
@@ -542,12 +548,12 @@ def int8_matmul_backward(dy, w, w_scales):
         _bad("weights must be int8 [N, K]")
     N, K = w.shape
     dev = dy.device
-    if dy.dim() < 1 or dy.shape[-1] != N:
-        _bad(f"dy {tuple(dy.shape)} must end in N={N}")
+    if dy.dim() < 1 or dy.shape[-1] != N or not N:
+        _bad(f"dy {tuple(dy.shape)} must end in N={N}, over 0")
     _i8_linear(N, K, dev, (w, w_scales))
     code = _i8_type(dy.dtype, "dy")
-    M = dy.numel() // N if N else 0
-    dx = torch.empty(dy.shape[:-1] + (K,), dtype=dy.dtype, device=dev)
+    M = dy.numel() // N
+    dx = _i8_out(dy, M, K, dy.dtype, dev)
     L = lib()
     _i8_call(L.mi_int8_matmul_backward, dev, L.mi_int8_backward_workspace(M, N, K, 1, code), dx.data_ptr(),
              dy.data_ptr(), w.data_ptr(), w_scales.data_ptr(), M, N, K, code)
@@ -561,15 +567,15 @@ def int8_gate_up_swiglu_backward(dy, gate, up, wg, sg, wu, su):
         _bad("weights must be int8 [N, K]")
     N, K = wg.shape
     dev = dy.device
-    if dy.dim() < 1 or dy.shape[-1] != N:
-        _bad(f"dy {tuple(dy.shape)} must end in N={N}")
+    if dy.dim() < 1 or dy.shape[-1] != N or not N:
+        _bad(f"dy {tuple(dy.shape)} must end in N={N}, over 0")
     for t in (gate, up):
         if t.shape != dy.shape or t.dtype != dy.dtype or t.device != dev:
             _bad("gate and up must match dy in shape, dtype and device")
     _i8_linear(N, K, dev, (wg, sg), (wu, su))
     code = _i8_type(dy.dtype, "dy")
-    M = dy.numel() // N if N else 0
-    dx = torch.empty(dy.shape[:-1] + (K,), dtype=dy.dtype, device=dev)
+    M = dy.numel() // N
+    dx = _i8_out(dy, M, K, dy.dtype, dev)
     dgate, dup = torch.empty_like(dy), torch.empty_like(dy)
     L = lib()
     _i8_call(L.mi_int8_gate_up_swiglu_backward, dev, L.mi_int8_backward_workspace(M, N, K, 2, code), dx.data_ptr(),

@@ -495,6 +495,19 @@ def test_leading_dimensions_and_empty(dev):
     assert mi_qmm.int8_matmul_backward(y[:0], w, sw).shape == (0, 64)
     with pytest.raises(mi_qmm.MiError):
         mi_qmm.int8_matmul_backward(y[:, :0].contiguous(), w[:0], sw[:0])
+    for call in (lambda: mi_qmm.int8_matmul(x.new_empty(2, 3, 0), w[:, :0].contiguous(), sw),
+                 lambda: mi_qmm.int8_matmul_backward(y.new_empty(2, 3, 0), w[:0], sw[:0]),
+                 lambda: mi_qmm.int8_quantize(x.new_empty(2, 0))):
+        with pytest.raises(mi_qmm.MiError):
+            call()
+    assert mi_qmm.int8_matmul(x.new_empty(2, 0, 64), w, sw).shape == (2, 0, 48)
+    assert mi_qmm.int8_matmul_backward(y.new_empty(0, 3, 48), w, sw).shape == (0, 3, 64)
+    q, s = mi_qmm.int8_quantize(x.view(2, 3, 64))
+    assert q.shape == (2, 3, 64) and s.shape == (2, 3) and mi_qmm.int8_quantize(x[0])[1].shape == ()
+    assert mi_qmm.int8_quantize(x.new_empty(2, 0, 64))[1].shape == (2, 0)
+    z = mi_qmm.int8_gate_up_swiglu(x.view(2, 3, 64), w, sw, w, sw, save=True)
+    dh = mi_qmm.int8_gate_up_swiglu_backward(z[0], z[1], z[2], w, sw, w, sw)
+    assert all(t.shape == (2, 3, 48) and t.is_contiguous() for t in z) and dh[0].shape == (2, 3, 64)
 
 
 def test_refusals_on_device(dev):
