@@ -15,7 +15,8 @@
 // What bounds it: large products the matrix cores and the DMA beside them at the clock that the card's
 // power allows: 8192 x 4096 x 14336 in 361 us, 2.66 POPS (a library product of the same codes: 402 to
 // 459 us, by their values); MFMA instructions are busy 67% of the time. 64-byte steps in a ring of
-// five stages took 444 us, weights straight into registers 455. Up to 256 rows or so the weights
+// five stages took 444 us, weights straight into registers 455, four waves of 128 x 128 each (a third
+// less read from LDS, one wave a SIMD) 444, 32 x 32 x 32 instructions 410. Up to 256 rows or so the weights
 // from HBM bound it: gate + up [14336,4096], 48 rows, 25.9 us (4.5 TB/s). Two things keep them coming:
 // - Rows of a power-of-two pitch meet in the same memory channels. Up to 256 rows a column tile starts
 //   3 steps further along K than the one before it and wraps round (int32 sums, exact in any
