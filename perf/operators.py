@@ -15,7 +15,6 @@ import sys
 import torch
 
 own = False
-_mi = None  # the library, once a call has needed it
 
 DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 
@@ -185,12 +184,11 @@ def run(st):
 
 
 def _library():
-    global _mi
-    if _mi is None:
-        sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "mlx-serve_amd"))
-        import mi_qmm
-        _mi = mi_qmm
-    return _mi
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "mlx-serve_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    import mi_qmm
+    return mi_qmm
 
 
 def work(case):
