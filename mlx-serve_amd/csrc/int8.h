@@ -43,9 +43,11 @@ struct Int8Params {
   bool vec16;  // their rows on 16 bytes
 };
 
-// dx[m,k] = row[m] * sum over banks, parts and n of a[m,n] w[n,k]: the scaled gradients a as fp16,
-// each row times a power of two (1 / row[m]) that puts its largest value into 2^14 .. 2^15, in
-// `terms` parts that add up: [(bank * terms + t)][M][np], zero from n = N on.
+// dx[m,k] = row[m] * sum over banks, parts and n of 2^(-11 t) a_t[m,n] w[n,k]: the scaled gradients as fp16,
+// each row times a power of two (1 / row[m]) that puts its largest value into 2^14 .. 2^15, in `terms`
+// parts, each of them what the one before it left times 2^11. The smallest part comes first:
+// [(terms - 1 - t) * banks + bank][M][np], zero from n = N on.
+constexpr int kPartBits = 11;
 struct Int8BwdParams {
   const uint16_t* a;
   const float* row;    // [M]

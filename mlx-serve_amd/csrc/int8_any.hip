@@ -128,7 +128,7 @@ hipError_t launch_token(const Int8Params& P, hipStream_t s) {
 }
 
 // dx: 64 rows x 64 codes of the weight rows' K; 32 values of n a step. The weights' tile is
-// turned in LDS (row k, values n) as exact fp16.
+// turned in LDS (row k, values n) as exact fp16, times the power of two of the gradients' part.
 constexpr int kLdB = 40;  // fp16 values of a staged row
 
 template <int T>
@@ -148,7 +148,8 @@ __global__ void __launch_bounds__(256) int8_bwd_any_kernel(Int8BwdParams P) {
   for (int i = 0; i < 4; ++i) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   for (int seg = 0; seg < P.banks * P.terms; ++seg) {
     const uint16_t* a = P.a + (int64_t)seg * P.M * P.np;
-    const int8_t* w = P.w[seg / P.terms];
+    const int8_t* w = P.w[seg % P.banks];
+    const float part = 1.f / (float)(1u << kPartBits * (P.terms - 1 - seg / P.banks));
     for (int n = 0; n < P.N; n += 32) {  // a is zero up to np, a multiple of 32
       *reinterpret_cast<u32x4_t*>(as + ar * kLdB + ac) =
           *reinterpret_cast<const u32x4_t*>(a + am * P.np + n + ac);
@@ -156,7 +157,8 @@ __global__ void __launch_bounds__(256) int8_bwd_any_kernel(Int8BwdParams P) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int k = k0 + wc + j;
-        const _Float16 f = on && k < P.K ? (_Float16)(float)w[(int64_t)(n + wr) * P.K + k] : (_Float16)0.f;
+        const _Float16 f = on && k < P.K ? (_Float16)((float)w[(int64_t)(n + wr) * P.K + k] * part)
+                                             : (_Float16)0.f;
         bs[(wc + j) * kLdB + wr] = __builtin_bit_cast(uint16_t, f);
       }
       __syncthreads();

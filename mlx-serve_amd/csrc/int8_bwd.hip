@@ -1,7 +1,8 @@
 // The gradient of an int8 product to its activations, on the matrix cores:
 //   dx[m,k] = row[m] * sum over n of a[m,n] w[n,k]
 // with the scaled gradients a in fp16 parts (int8_quant.hip) and the codes as exact fp16, fp32
-// sums; the banks and parts follow one another along the sum.
+// sums; the parts follow one another along the sum, smallest first and the banks within each. A part's
+// power of two goes into the codes as they become fp16.
 //
 // Block: 8 waves as 2 (rows of a) x 4 (columns of w), BM x BN outputs, v_mfma_f32_16x16x32_f16 with
 // D[k][m] = w[n][k] a[m][n]. A step is 64 values of n: rows of a are one cache line, the codes 64
@@ -10,7 +11,8 @@
 // fragment takes one column of eight rows: ds_read_b64_tr_b8 gives lane l of 16 column l % 16 of the
 // 8 x 16 bytes that the 16 lanes point at, so w is read as it lies in memory, and no turned copy of
 // it is made. Codes become fp16 in registers, five operations for four: u = code + 128 in the low
-// byte of 0x64 is 1024 + u, minus 1152.
+// byte of 0x64 is 1024 + u, minus 1152; an exponent of 11 less in both is 2^-11 of that, and 22 less 2^-22
+// (subnormal, and exact).
 //
 // What bounds it: the matrix cores at the clock that the card's power allows. dx [4096,4096] of gate
 // + up [14336,4096] takes 686 us behind the gradient's pass, 1.40 PFLOP/s, where a bf16 library product
@@ -43,12 +45,20 @@ MI_DEV int nswz(int n) {
   return BN == 256 ? (n & 7) | ((n >> 1) & 8) : ((n >> 1) & 3) | ((n >> 2) & 4);
 }
 
+// The fp16 exponent that codes come under, and what is taken off again (1152 of their unit), for part t of
+// the gradients.
+struct CodeUnit {
+  uint32_t c, off;
+  MI_DEV explicit CodeUnit(int t) : c(0x64646464u - t * 0x2C2C2C2Cu), off(0xE480E480u - t * 0x2C002C00u) {}
+};
+static_assert(kPartBits == 0x2C / 4, "a part's bits in fp16's exponent");
+
 // four codes -> fp16, in order
-MI_DEV u32x2_t codes_f16(uint32_t w) {
-  const uint32_t u = w ^ 0x80808080u, c = 0x64646464u;
-  const f16x2_t off = {(_Float16)-1152.f, (_Float16)-1152.f};
-  const f16x2_t a = __builtin_bit_cast(f16x2_t, perm_b32(c, u, 0x04010400u)) + off;
-  const f16x2_t b = __builtin_bit_cast(f16x2_t, perm_b32(c, u, 0x04030402u)) + off;
+MI_DEV u32x2_t codes_f16(uint32_t w, const CodeUnit& unit) {
+  const uint32_t u = w ^ 0x80808080u;
+  const f16x2_t off = __builtin_bit_cast(f16x2_t, unit.off);
+  const f16x2_t a = __builtin_bit_cast(f16x2_t, perm_b32(unit.c, u, 0x04010400u)) + off;
+  const f16x2_t b = __builtin_bit_cast(f16x2_t, perm_b32(unit.c, u, 0x04030402u)) + off;
   return u32x2_t{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
 }
 
@@ -79,7 +89,8 @@ int8_bwd_kernel(Int8BwdParams P) {
   const TileOf at = tile_of_block(mtiles, P.ct1 - P.ct0);
   const int m0 = at.mt * BM, k0 = (P.ct0 + at.nt) * BN, s0 = at.split * P.sps;
   const int seg_steps = np / kBN_;
-  const int ns = min(P.sps, P.banks * P.terms * seg_steps - s0);
+  const int part_steps = P.banks * seg_steps;
+  const int ns = min(P.sps, P.terms * part_steps - s0);
   const int mrows = min(BM, M - m0);
   const int abytes = mrows * np * 2;
 
@@ -96,7 +107,7 @@ int8_bwd_kernel(Int8BwdParams P) {
     const int c = 16 * ((lane % (BN / 16)) ^ nswz<BN>(wr[i]));
     wo[i] = k0 + c < ldw ? (uint32_t)wr[i] * (uint32_t)ldw + (uint32_t)(k0 + c) : kOOB;
   }
-  // where a stage reads: part `seg`, values n .. n + 63 of it
+  // where a stage reads: bank and part `seg`, values n .. n + 63 of it
   struct Cursor {
     int st, seg, n;
   };
@@ -113,7 +124,7 @@ int8_bwd_kernel(Int8BwdParams P) {
     }
   };
   auto abase = [&](const Cursor& c) { return P.a + ((size_t)c.seg * M + m0) * np; };
-  auto wbase = [&](const Cursor& c) { return P.w[c.seg >= P.terms] + (size_t)c.n * ldw; };
+  auto wbase = [&](const Cursor& c) { return P.w[c.seg & (P.banks - 1)] + (size_t)c.n * ldw; };
   // stages past the range load through resources of zero records (zeros, no traffic), rows from N
   // on and columns from K on out of bounds
   auto issue = [&](const Cursor& c, int slot, int j) __attribute__((always_inline)) {  // instruction j
@@ -147,14 +158,16 @@ int8_bwd_kernel(Int8BwdParams P) {
   auto read_x = [&](int slot, int e, int i) __attribute__((always_inline)) {
     X[e][i] = *reinterpret_cast<const u32x4_t*>(smem + slot * kStage + xr + (e ? fo1 : fo0) + 16 * i * 128);
   };
-  auto to_f16 = [&](int e, int a) -> u32x4_t {
-    const u32x2_t lo = codes_f16((uint32_t)A[e][a].x), hi = codes_f16((uint32_t)A[e][a].y);
+  auto to_f16 = [&](int e, int a, const CodeUnit& u) -> u32x4_t {
+    const u32x2_t lo = codes_f16((uint32_t)A[e][a].x, u), hi = codes_f16((uint32_t)A[e][a].y, u);
     return u32x4_t{lo.x, lo.y, hi.x, hi.y};
   };
   // The products of half e, one tile of codes at a time. Beside a tile's MFMAs: the next tile's
   // codes to fp16, and a part of the next half's fragment reads (its codes first: the last tile's
-  // neighbour is their first) from stage `rs`, and of the DMA where `dma`.
-  auto half = [&](int e, int rs, bool dma, const Cursor& c, int slot) __attribute__((always_inline)) {
+  // neighbour is their first) from stage `rs`, and of the DMA where `dma`. Codes of this stage in unit
+  // `u`, of the next half's in `un`.
+  auto half = [&](int e, int rs, bool dma, const Cursor& c, int slot, const CodeUnit& u, const CodeUnit& un)
+                  __attribute__((always_inline)) {
     constexpr int kX = NT > 1 ? (MT + NT - 2) / (NT - 1) : MT;  // x reads of the tiles after the first
 #pragma unroll
     for (int a = 0; a < NT; ++a) {
@@ -166,7 +179,7 @@ int8_bwd_kernel(Int8BwdParams P) {
 #pragma unroll
         for (int j = a; j < XI + WI; j += NT) issue(c, slot, j);
       }
-      Wf[(a + 1) & 1] = a + 1 < NT ? to_f16(e, a + 1) : to_f16(e ^ 1, 0);
+      Wf[(a + 1) & 1] = a + 1 < NT ? to_f16(e, a + 1, u) : to_f16(e ^ 1, 0, un);
 #pragma unroll
       for (int i = 0; i < MT; ++i) acc[a][i] = mfma_f16(Wf[a & 1], X[e][i], acc[a][i]);
 #pragma unroll
@@ -195,17 +208,27 @@ int8_bwd_kernel(Int8BwdParams P) {
   read_a(0, 0);
 #pragma unroll
   for (int i = 0; i < MT; ++i) read_x(0, 0, i);
-  Wf[0] = to_f16(0, 0);
+  const int order = s0 / part_steps;                // parts before this range's first
+  int end = (order + 1) * part_steps - s0;          // of its steps
+  CodeUnit unit(P.terms - 1 - order);
+  Wf[0] = to_f16(0, 0, unit);
   int slot = 0;
 #pragma unroll 1
   for (int t = 0; t < ns; ++t) {
     const int next = slot + 1 == R ? 0 : slot + 1;
-    half(0, slot, false, ci, slot);
+    CodeUnit ahead = unit;  // the next step's
+    if (t + 1 == end) {
+      ahead.c += 0x2C2C2C2Cu;
+      ahead.off += 0x2C002C00u;
+      end += part_steps;
+    }
+    half(0, slot, false, ci, slot, unit, unit);
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): this wave's reads of stage t
     wait_vm((R - 2) * (XI + WI));
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
-    half(1, next, true, ci, slot);
+    half(1, next, true, ci, slot, unit, ahead);
+    unit = ahead;
     step(ci);
     slot = next;
   }

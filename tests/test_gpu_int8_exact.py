@@ -1,0 +1,53 @@
+"""The int8 operators on data with one right answer (int8_exact.py), and in the kernels that the other sizes miss."""
+import pytest
+import torch
+
+import int8_exact as X
+import int8_ref as R
+import mi_qmm
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+TYPES = [BF16, F16, F32]
+
+
+def _case(**kw):
+    print("CASE", kw, flush=True)
+
+
+def _off(t, n):
+    """The same values n elements behind a 16-byte boundary."""
+    v = torch.empty(t.numel() + n, dtype=t.dtype, device="cuda")[n:].view(t.shape)
+    v.copy_(t)
+    return v
+
+
+def _within(y, ref, tol, what):
+    over = (y.double() - ref).abs() - tol
+    assert torch.isfinite(y).all() and over.max().item() <= 0, f"{what}: {over.max().item():.3g} over the bound"
+
+
+# ------------------------------------------------ what a scaled gradient keeps --
+@pytest.mark.parametrize("M,N", [(1, 16), (5, 48), (130, 208), (300, 1000)])
+def test_fp32_gradients_keep_22_bits(dev, M, N):
+    """Down to 2^-28 of their row's largest value."""
+    _case(t="wide", M=M, N=N)
+    dy, w, s = X.wide_case(M, N, 28, "cuda")
+    ref = dy.double() @ w.double()
+    for what, args in (("aligned", (dy, w, s)), ("off", (_off(dy, 1), _off(w, 3), s))):
+        _within(mi_qmm.int8_matmul_backward(*args), ref, 2.0 ** -22 * ref.abs(), what)
+
+
+@pytest.mark.parametrize("M,N", [(5, 48), (130, 208)])
+def test_banks_of_unlike_scales(dev, M, N):
+    """dup's scales 2^-24 of dgate's: its part of dx keeps 22 bits, though both share a row's power of two."""
+    dy, w, s = X.wide_case(M, N, 3, "cuda")
+    z = torch.zeros_like(w)
+    gate, up = torch.full_like(dy, 64.0), torch.ones_like(dy)
+    wg, wu = torch.cat([w, z], 1), torch.cat([z, w], 1)
+    su = s * 2.0 ** -30
+    dx, dg, du = mi_qmm.int8_gate_up_swiglu_backward(dy, gate, up, wg, s, wu, su)
+    assert torch.equal(dg, dy) and torch.equal(du, 64 * dy)
+    ref = torch.cat([dy.double() @ w.double(), (64 * dy.double() * su.double()) @ w.double()], 1)
+    _within(dx, ref, 2.0 ** -22 * ref.abs(), "dx")
