@@ -149,15 +149,14 @@ int forward(mi::Int8Params& P, const void* x, const float* x_scales, int64_t M, 
                     "int8 matmul launch");
 }
 
-// Backward workspace: the fp16 parts of the scaled gradients, [banks * terms][M][np] (two parts for
-// fp32, one otherwise), the rows' powers of two, the codes in rows of ldw where K is no multiple of
-// 16, then the ranges' sums of a split product.
+// Backward workspace: the fp16 parts of the scaled gradients, [terms * banks][M][np], the rows' powers of two,
+// the codes in rows of ldw where K is no multiple of 16, then the ranges' sums of a split product.
 int64_t parts_bytes(const mi::Int8BwdParams& B) { return up((int64_t)B.banks * B.terms * B.M * B.np * 2, 256); }
 int64_t rows_bytes(const mi::Int8BwdParams& B) { return up((int64_t)B.M * 4, 256); }
 int64_t backward_need(mi::Int8BwdParams& B, int64_t M, int64_t N, int64_t K, int banks, int type) {
   if (M == 0 || N == 0 || K == 0) return 0;
   B.banks = banks;
-  B.terms = type == mi::kF32 ? 2 : 1;
+  B.terms = mi::kParts;
   B.np = (int)up(N, 64);
   B.M = (int)M;
   B.N = (int)N;

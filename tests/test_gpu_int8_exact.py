@@ -51,3 +51,16 @@ def test_banks_of_unlike_scales(dev, M, N):
     assert torch.equal(dg, dy) and torch.equal(du, 64 * dy)
     ref = torch.cat([dy.double() @ w.double(), (64 * dy.double() * su.double()) @ w.double()], 1)
     _within(dx, ref, 2.0 ** -22 * ref.abs(), "dx")
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("M,N", [(3, 32), (130, 400), (300, 2080)])
+def test_differences_of_products(dev, M, N, t):
+    """Two products a column that nearly cancel: 22 bits of each."""
+    _case(t="differences", M=M, N=N, type=t)
+    dy, w, s = X.cancelling_case(M, N, t, "cuda")
+    ref, tol = X.cancelling_sum(dy, w, s, 2.0 ** -22)
+    for what, args in (("aligned", (dy, w, s)), ("off", (_off(dy, 1), _off(w, 3), s))):
+        _within(mi_qmm.int8_matmul_backward(*args), ref, tol, what)
+    gate, up, z = torch.full_like(dy, 64.0), torch.ones_like(dy), torch.zeros_like(w)
+    _within(mi_qmm.int8_gate_up_swiglu_backward(dy, gate, up, w, s, z, s / 64)[0], ref, tol, "gate + up")
