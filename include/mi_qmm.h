@@ -327,8 +327,9 @@ int mi_int8_gate_up_swiglu(void* y, void* gate, void* up, const void* x, const f
 /* The gradient of mi_int8_matmul to its activations: dx[m,k] = sum_n dy[m,n] w_scales[n] w[n,k].
  * Weights and scales are constants (a frozen base under adapters), and the rounding of the
  * activations is passed straight through. dy [M, N] and dx [M, K] in dtype (bfloat16, float16 or
- * float32), fp32 sums. Each dy * scale enters the sum with 22 bits down to 2^-28 of its row's largest, and
- * with an error of 2^-50 of that largest below; of gate + up, the row's largest of both projections. */
+ * float32), fp32 sums. Each dy * scale, rounded to fp32, enters the sum with 22 bits (float32: all 24)
+ * down to 2^-28 of its row's largest, and with an error of 2^-49 of that largest below; of gate + up, the
+ * row's largest of both projections. */
 int mi_int8_matmul_backward(void* dx, const void* dy, const int8_t* w, const float* w_scales,
                             int64_t M, int64_t N, int64_t K, int dtype, void* workspace,
                             int64_t workspace_bytes, void* stream);

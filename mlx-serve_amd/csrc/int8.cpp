@@ -156,7 +156,7 @@ int64_t rows_bytes(const mi::Int8BwdParams& B) { return up((int64_t)B.M * 4, 256
 int64_t backward_need(mi::Int8BwdParams& B, int64_t M, int64_t N, int64_t K, int banks, int type) {
   if (M == 0 || N == 0 || K == 0) return 0;
   B.banks = banks;
-  B.terms = mi::kParts;
+  B.terms = mi::int8_parts(type);
   B.np = (int)up(N, 64);
   B.M = (int)M;
   B.N = (int)N;

@@ -48,7 +48,7 @@ struct Int8Params {
 // parts, each of them what the one before it left times 2^11. The smallest part comes first:
 // [(terms - 1 - t) * banks + bank][M][np], zero from n = N on.
 constexpr int kPartBits = 11;
-constexpr int kParts = 2;
+__host__ __device__ constexpr int int8_parts(int type) { return type == kF32 ? 3 : 2; }
 struct Int8BwdParams {
   const uint16_t* a;
   const float* row;    // [M]

@@ -149,13 +149,15 @@ hipError_t launch_type(int8_t* q, float* s, const void* x, int64_t rows, int64_t
 }
 
 // ------------------------------------------------------------- SwiGLU gradient ---
-// The values that the backward product sums, times their channel scale, as two fp16 parts of 11 bits. (The
-// scale alone has 24 bits: one part adds 2^-11 of a value to a sum of values that may cancel, and half as
-// much again to the error of an fp16 result: 2.9e-4 of its norm, 2.1e-4 with two.) fp16's range is met by
-// a power of two for each row, exact both ways: the row's largest value goes into 2^14 .. 2^15. The second
-// part is times 2^11, so that it has 11 bits wherever the first does: the two leave 2^-22 of a value down
-// to 2^-28 of the row's largest, and 2^-50 of that largest below. A row with an infinity or a NaN is
-// taken as it is.
+// The values that the backward product sums, times their channel scale, as fp16 parts of 11 bits: two, and three where
+// the gradient is fp32, which keep its 24. (The scale alone has 24 bits: one part adds 2^-11 of a value to a sum
+// of values that may cancel, and half as much again to the error of an fp16 result: 2.9e-4 of its norm,
+// 2.1e-4 with two.) fp16's range is met by a power of two for each row, exact both ways: the row's
+// largest value goes into 2^14 .. 2^15. Each part is what the one before left, times 2^11, so that it
+// has 11 bits wherever the first does: two leave 2^-22 of a value down to 2^-28 of the row's largest, and 2^-50
+// of that largest below; three leave nothing of an fp32 value down to 2^-28 (below, where the first part is
+// subnormal, the matrix instructions cut the others off at 2^-51). A row with an infinity or a NaN is taken as
+// it is.
 //
 // Memory-bound (three reads, four writes of [M, N] with both outputs); a row is held in
 // registers between its maximum and the parts. Measured: [4096,14336] bf16 gate + up 160 us, 5.1 TB/s.
@@ -247,7 +249,7 @@ MI_DEV void pack_store(void* p, int64_t v, const float (&f)[E]) {
 // A block a row, VPT vectors of 16 bytes a thread; np / E vectors of `a` a row.
 template <int T, int BANKS, int WPR, int VPT>
 __global__ void __launch_bounds__(WPR * 64) int8_grad_kernel(Int8GradParams P) {
-  constexpr int E = T == kF32 ? 4 : 8, TERMS = kParts;
+  constexpr int E = T == kF32 ? 4 : 8, TERMS = int8_parts(T);
   __shared__ uint32_t part[WPR];
   const int64_t m = blockIdx.x;
   const int nv = P.N / E, npv = P.np / E;
@@ -325,7 +327,7 @@ __global__ void __launch_bounds__(WPR * 64) int8_grad_kernel(Int8GradParams P) {
 // Any width and alignment: a block a row, which is read and computed twice.
 template <int T, int BANKS>
 __global__ void __launch_bounds__(256) int8_grad_any_kernel(Int8GradParams P) {
-  constexpr int TERMS = kParts;
+  constexpr int TERMS = int8_parts(T);
   __shared__ uint32_t part[4];
   for (int64_t m = blockIdx.x; m < P.M; m += gridDim.x) {
     const int64_t at = m * P.N;

@@ -39,6 +39,25 @@ def test_fp32_gradients_keep_22_bits(dev, M, N):
         _within(mi_qmm.int8_matmul_backward(*args), ref, 2.0 ** -22 * ref.abs(), what)
 
 
+@pytest.mark.parametrize("M,N", [(1, 16), (5, 48), (130, 208), (300, 1000)])
+def test_fp32_gradients_keep_all_bits(dev, M, N):
+    """24 bits of each value down to 2^-28 of their row's largest, in a row that goes down to 2^-37.
+
+    Below 2^-28 the first part is subnormal. The matrix instruction adds what the smaller parts gave to a product
+    that it places by the smallest normal exponent, less than 2 x 2^-14 |w|; of what is added 24 bits from there
+    stay, which cuts off less than 2^-37 |w|. The row's largest is 2^14 at least: 2^-51 |w| of it. The second part
+    does the same 2^-11 lower, and 2^-61 was not kept at all: 2^-50 in all."""
+    _case(t="all bits", M=M, N=N)
+    dy, w, s = X.wide_case(M, N, 37, "cuda")
+    ref = dy.double() @ w.double()
+    top = dy.abs().amax(1, keepdim=True)
+    small = dy.abs() < top * 2.0 ** -28  # (w is a diagonal: column k has dy[:, k])
+    tol = torch.where(small, 2.0 ** -50 * top.double() * w.double().abs().sum(0), 0.0)
+    assert small.sum() < 0.4 * small.numel()
+    for what, args in (("aligned", (dy, w, s)), ("off", (_off(dy, 1), _off(w, 3), s))):
+        _within(mi_qmm.int8_matmul_backward(*args), ref, tol, what)
+
+
 @pytest.mark.parametrize("M,N", [(5, 48), (130, 208)])
 def test_banks_of_unlike_scales(dev, M, N):
     """dup's scales 2^-24 of dgate's: its part of dx keeps 22 bits, though both share a row's power of two."""
