@@ -317,7 +317,8 @@ int mi_int8_matmul(void* y, const void* x, const float* x_scales, const int8_t* 
                    int x_dtype, int y_dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* y = silu(g) * u with g and u the products of x with w_gate and w_up (as mi_int8_matmul),
- * silu(g) = g / (1 + e^-g) in fp32, one rounding. gate and up: both NULL, or [M, N] in y's type
+ * silu(g) = g / (1 + e^-g) in fp32 (where y is bfloat16 or float16 the exponential is good to
+ * (5 + 1.25 |g|) 2^-24, below their own last bit), one rounding. gate and up: both NULL, or [M, N] in y's type
  * for g and u, each rounded once, as the backward pass takes them. */
 int mi_int8_gate_up_swiglu(void* y, void* gate, void* up, const void* x, const float* x_scales,
                            const int8_t* w_gate, const float* s_gate, const int8_t* w_up,
@@ -335,7 +336,7 @@ int mi_int8_matmul_backward(void* dx, const void* dy, const int8_t* w, const flo
                             int64_t workspace_bytes, void* stream);
 
 /* The gradients of mi_int8_gate_up_swiglu: with s = 1 / (1 + e^-g),
- *   dgate = dy * u * s * (1 + g (1 - s)),   dup = dy * g * s   (fp32, one rounding each)
+ *   dgate = dy * u * s * (1 + g (1 - s)),   dup = dy * g * s   (fp32, s as in the forward call, one rounding each)
  *   dx[m,k] = sum_n dgate[m,n] s_gate[n] w_gate[n,k] + dup[m,n] s_up[n] w_up[n,k]
  * from gate and up as the forward call gave them; dx is formed from dgate and dup before their
  * rounding, otherwise as mi_int8_matmul_backward. dgate and dup ([M, N], both or neither NULL)

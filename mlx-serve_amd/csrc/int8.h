@@ -182,13 +182,25 @@ MI_DEV f32x4_t mfma_f16(u32x4_t a, u32x4_t b, f32x4_t c) {
                                                 __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
 }
 
-// 1 / (1 + e^-g) on the hardware's exponential and reciprocal, one ulp each, and |g| / 2^24 from
-// rounding the exponent (with the library's exponential and a correctly rounded quotient, five times
-// the instructions, 2003 rows of gate + up [14336,4096] took 290 us against 281). e^-g overflows to infinity for g < -88, which
-// gives 0, the limit.
-MI_DEV float sigmoid_f(float g) {
-  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * g));
+// s = 1 / (1 + e^-g), and 1 - s.
+struct Sigmoid {
+  float s, c;
+};
+// For results of 8 or 11 bits, on the hardware's exponential and reciprocal: one ulp each, and 1.25 |g| / 2^24
+// from rounding the exponent, 2^-17 in all up to |g| = 88, where a result's own rounding is 2^-11 at best.
+// e^-g overflows to infinity for g < -88, which gives 0, the limit. (sigmoid_f32 in its place, five times the
+// instructions, took 2003 rows of gate + up [14336,4096] from 281 to 290 us.)
+MI_DEV Sigmoid sigmoid_16(float g) {
+  const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * g));
+  return {s, 1.f - s};
 }
+// For fp32 results: e = e^-|g| has no large argument and does not overflow, and neither s nor 1 - s
+// comes of a difference. e is good to one ulp, the sum, quotient and product round once each.
+MI_DEV Sigmoid sigmoid_f32(float g) {
+  const float e = expf(-fabsf(g)), t = 1.f / (1.f + e);
+  return g < 0.f ? Sigmoid{e * t, t} : Sigmoid{t, e * t};
+}
+MI_DEV Sigmoid sigmoid_of(float g, bool f32) { return f32 ? sigmoid_f32(g) : sigmoid_16(g); }
 
 // Four neighbouring values, one rounding each; `vec`: with one store.
 MI_DEV void store4(void* p, int64_t i, int type, bool vec, int cnt, const float (&v)[4]) {
@@ -247,7 +259,7 @@ MI_DEV void scaled4(const Int8Params& P, i32x4_t a, i32x4_t b, float sx, const C
     g[j] = (float)a[j] * sx * c.s[j];
     if constexpr (DUAL) {
       u[j] = (float)b[j] * sx * c.s2[j];
-      y[j] = g[j] * sigmoid_f(g[j]) * u[j];
+      y[j] = g[j] * sigmoid_of(g[j], P.type == kF32).s * u[j];
     } else {
       y[j] = P.bias ? g[j] + c.b[j] : g[j];
     }

@@ -196,9 +196,9 @@ MI_DEV Grad<T> gradient(float dy, float g, float u, float sw, float sw2) {
     r.a = dy * sw;
     r.b = r.dg = r.du = 0.f;
   } else {
-    const float sig = sigmoid_f(g);
-    r.dg = dy * u * sig * (1.f + g * (1.f - sig));
-    r.du = dy * g * sig;
+    const Sigmoid sig = sigmoid_of(g, T == kF32);
+    r.dg = dy * u * sig.s * (1.f + g * sig.c);
+    r.du = dy * g * sig.s;
     r.a = r.dg * sw;
     r.b = r.du * sw2;
   }

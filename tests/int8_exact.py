@@ -66,3 +66,44 @@ def cancelling_sum(dy, w, s, left):
     mag = a.abs() @ w.double().abs()
     dx = a @ w.double()
     return dx, 1.01 * (HALF[dy.dtype] * dx.abs() + mag * (left + U + 12 * U)) + FLOOR[dy.dtype]
+
+
+# ---------------------------------------------------------------- the fp32 sigmoid --
+# s = 1 / (1 + e) or e / (1 + e), e = exp(-|g|) to one ulp (2 U), the sum, the quotient and the product U each:
+# 6 U at most. An e below 2^-126 is off by a subnormal step at most.
+SIG = 6 * U
+STEP = 2.0 ** -148
+
+
+def silu_case(device):
+    """Codes whose gate is a b / 128 exactly, -126 .. 126, and whose up is a power of two up to 2^100."""
+    a = torch.arange(-127, 128, device=device)
+    b = torch.arange(1, 128, 2, device=device)
+    x = torch.zeros(a.numel(), 16, dtype=torch.int8, device=device)
+    x[:, 0], x[:, 1] = a.to(torch.int8), 1
+    wg = torch.zeros(b.numel(), 16, dtype=torch.int8, device=device)
+    wu = wg.clone()
+    wg[:, 0], wu[:, 1] = b.to(torch.int8), 1
+    sg = torch.full((b.numel(),), 2.0 ** -7, device=device)
+    su = torch.exp2((b % 4).float() / 3 * 100).clamp(max=2.0 ** 100)
+    su = torch.exp2(torch.log2(su).round())
+    return x, torch.ones(a.numel(), device=device), wg, sg, wu, su
+
+
+def silu(x, wg, sg, wu, su):
+    """(y, bound) of silu_case: two products more than the sigmoid."""
+    g, u = (x.double() @ w.double().t() * s.double() for w, s in ((wg, sg), (wu, su)))
+    y = g * torch.special.expit(g) * u
+    return y, 1.01 * (SIG + 2 * U) * y.abs() + (g * u).abs() * STEP + FLOOR[F32]
+
+
+def dsilu(dy, g, u):
+    """(dgate, dup, bounds): s and 1 - s to SIG each; dgate = ((dy u) s) (1 + g (1 - s)). Where (dy u) s is
+    subnormal it rounds by half a step, 2^-150, which the last factor multiplies."""
+    dy, g, u = dy.double(), g.double(), u.double()
+    s, c = torch.special.expit(g), torch.special.expit(-g)
+    f = 1 + g * c
+    dg, du = dy * u * s * f, dy * g * s
+    tg = (dy * u * s).abs() * ((g * c).abs() * (SIG + U) + f.abs() * (SIG + 4 * U))
+    return (dg, du, 1.01 * tg + (dy * u).abs() * (1 + g.abs()) * STEP + (1 + f.abs()) * FLOOR[F32],
+            1.01 * du.abs() * (SIG + 3 * U) + (dy * g).abs() * STEP + FLOOR[F32])

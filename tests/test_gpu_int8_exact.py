@@ -83,3 +83,25 @@ def test_differences_of_products(dev, M, N, t):
         _within(mi_qmm.int8_matmul_backward(*args), ref, tol, what)
     gate, up, z = torch.full_like(dy, 64.0), torch.ones_like(dy), torch.zeros_like(w)
     _within(mi_qmm.int8_gate_up_swiglu_backward(dy, gate, up, w, s, z, s / 64)[0], ref, tol, "gate + up")
+
+
+# ------------------------------------------------------------------- the sigmoid --
+def test_silu_in_fp32(dev):
+    x, sx, wg, sg, wu, su = X.silu_case("cuda")
+    ref, tol = X.silu(x, wg, sg, wu, su)
+    for m in (1, 40, x.shape[0]):
+        y = mi_qmm.int8_gate_up_swiglu(x[:m].contiguous(), wg, sg, wu, su, x_scales=sx[:m].contiguous(), dtype=F32)
+        _within(y, ref[:m], tol[:m], m)
+
+
+def test_silu_gradient_in_fp32(dev):
+    g = torch.cat([torch.arange(-6400, 6400, device="cuda").float() / 64, torch.tensor([-1.2784645, 0.0], device="cuda")])
+    gate = torch.cat([g, g[:14]]).view(-1, 16)  # 801 rows
+    r = X.gen(1, "cuda")
+    dy, up = (torch.randn(gate.shape, device="cuda", generator=r) for _ in range(2))
+    w, s = torch.ones(16, 32, dtype=torch.int8, device="cuda"), torch.ones(16, device="cuda")
+    ref_g, ref_u, tol_g, tol_u = X.dsilu(dy, gate, up)
+    for args in ((dy, gate, up), (_off(dy, 1), gate, up)):
+        _, dg, du = mi_qmm.int8_gate_up_swiglu_backward(*args, w, s, w, s)
+        _within(dg, ref_g, tol_g, "dgate")
+        _within(du, ref_u, tol_u, "dup")
