@@ -30,6 +30,66 @@ def rounded(v, t):
     return v.float().to(t)
 
 
+# ------------------------------------------------------------ sums that are exact --
+def _dense(g, M, N, K, device):
+    """Three bits a value, every code: each term counts."""
+    dy = _ints(g, (M, N), -3, 3, device).float()
+    w = [_ints(g, (N, K), -127, 127, device).to(torch.int8) for _ in range(2)]
+    return dy, w, [_powers(g, N, -9, -8, device) for _ in range(2)]
+
+
+def _sparse(g, M, N, K, t, banks, device):
+    """Values and scales whose products have 20 bits (24 of one fp32 value), few codes a column: each bit counts."""
+    top, s_top = {torch.bfloat16: (255, 4095), torch.float16: (2047, 511), torch.float32: ((1 << 24) - 1, 1)}[t]
+    dy = _ints(g, (M, N), -top, top, device).float()
+    s = _ints(g, (N,), s_top // 2 + 1, s_top, device).float() * 2.0 ** -9
+    w = [torch.zeros(N, K, dtype=torch.int8, device=device) for _ in range(banks)]
+    k = torch.arange(K, device=device)
+    terms = 1 if t == F32 else 4
+    for b in range(banks):
+        for j in range(terms):
+            c = _ints(g, (K,), 1, 4 // banks if terms > 1 else 1, device) * (1 - 2 * _ints(g, (K,), 0, 1, device))
+            if terms == 1:
+                c = c * (k % banks == b)
+            w[b][(N - 1 - k - j * (N // 4)) % N, k] += c.to(torch.int8)  # (rows of a column meet where N < 4: c adds up)
+    return dy, w, [s] * banks
+
+
+def product_case(M, N, K, t, dense, device, seed=0):
+    """(dy, w, scales)"""
+    g = gen(seed + M + 3 * N + 7 * K, device)
+    dy, w, s = _dense(g, M, N, K, device) if dense else _sparse(g, M, N, K, t, 1, device)
+    return dy.to(t), w[0], s[0]
+
+
+def gated_case(M, N, K, t, dense, device, seed=0):
+    """(dy, gate, up, w, scales) of two banks. gate = 64, where the sigmoid is 1 in fp32 and its derivative nothing
+    beside 1, so that dgate = dy up and dup = 64 dy: integers again."""
+    g = gen(seed + M + 3 * N + 7 * K, device)
+    dy, w, s = _dense(g, M, N, K, device) if dense else _sparse(g, M, N, K, t, 2, device)
+    up = _powers(g, M * N, 0, 1 if dense else 0, device).view(M, N)
+    return dy.to(t), torch.full((M, N), 64.0, device=device).to(t), up.to(t), w, [s[0], s[1] / 64]
+
+
+def exact_sum(a, w):
+    """sum over the banks of a @ w (a: the scaled gradients) in 64 bits, where every partial sum is a whole multiple of
+    2^-9 below 2^24 of them."""
+    mag = sum(v.double().abs() @ c.double().abs() for v, c in zip(a, w))
+    assert mag.max().item() < 2.0 ** 15
+    assert all(torch.equal(v * 512, (v * 512).round()) for v in a)
+    return sum(v.double() @ c.double() for v, c in zip(a, w))
+
+
+def scaled(d, s):
+    return [x.double() * y.double() for x, y in zip(d, s)]
+
+
+def rounded(v, t):
+    """Values that fp32 holds, in 64 bits, as t."""
+    assert torch.equal(v.float().double(), v)
+    return v.float().to(t)
+
+
 # ------------------------------------------------------- what a value keeps of its bits --
 def wide_case(M, N, span, device, seed=0):
     """fp32 rows whose values have 24 bits and lie between the row's largest and 2^-span of it; one code a column, a

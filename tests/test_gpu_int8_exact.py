@@ -85,6 +85,38 @@ def test_differences_of_products(dev, M, N, t):
     _within(mi_qmm.int8_gate_up_swiglu_backward(dy, gate, up, w, s, z, s / 64)[0], ref, tol, "gate + up")
 
 
+# ------------------------------------------------------ sums with one right answer --
+# Every tile of the product, with and without ranges of the sum, and the small tiles behind whole rounds of big ones, for
+# each count of banks and parts; rows, columns and the sum end inside tiles and steps.
+EXACT = [(18, 36, 65), (1477, 119, 65), (2103, 34, 337), (2716, 652, 72), (2719, 656, 130), (66, 8650, 838),
+         (70, 8656, 900), (2091, 1940, 193), (2091, 1944, 200), (129, 3278, 5450), (129, 3280, 5452), (150, 6551, 6739),
+         (2712, 8553, 194), (2712, 8560, 200), (667, 4100, 4096), (1000, 2048, 5632), (512, 14336, 4096),
+         (1024, 4096, 14336)]
+
+
+@pytest.mark.parametrize("dense", [True, False])
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("M,K,N", EXACT)
+def test_exact_product_gradients(dev, M, K, N, t, dense):
+    _case(t="exact", M=M, K=K, N=N, type=t, dense=dense)
+    dy, w, s = X.product_case(M, N, K, t, dense, "cuda")
+    want = X.rounded(X.exact_sum(X.scaled([dy], [s]), [w]), t)
+    assert torch.equal(mi_qmm.int8_matmul_backward(dy, w, s), want)
+
+
+@pytest.mark.parametrize("dense", [True, False])
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("M,K,N", EXACT)
+def test_exact_gated_gradients(dev, M, K, N, t, dense):
+    _case(t="exact gated", M=M, K=K, N=N, type=t, dense=dense)
+    dy, gate, up, w, s = X.gated_case(M, N, K, t, dense, "cuda")
+    d = [dy.double() * up.double(), dy.double() * 64]
+    want = X.rounded(X.exact_sum(X.scaled(d, s), w), t)
+    dx, dg, du = mi_qmm.int8_gate_up_swiglu_backward(dy, gate, up, w[0], s[0], w[1], s[1])
+    assert torch.equal(dx, want)
+    assert torch.equal(dg, X.rounded(d[0], t)) and torch.equal(du, X.rounded(d[1], t))
+
+
 # ------------------------------------------------------------------- the sigmoid --
 def test_silu_in_fp32(dev):
     x, sx, wg, sg, wu, su = X.silu_case("cuda")
