@@ -1,4 +1,6 @@
 """The int8 operators on data with one right answer (int8_exact.py), and in the kernels that the other sizes miss."""
+import math
+
 import pytest
 import torch
 
@@ -137,3 +139,74 @@ def test_silu_gradient_in_fp32(dev):
         _, dg, du = mi_qmm.int8_gate_up_swiglu_backward(*args, w, s, w, s)
         _within(dg, ref_g, tol_g, "dgate")
         _within(du, ref_u, tol_u, "dup")
+
+
+# ---------------------------------------------- kernels that other sizes miss --
+def _codes(M, N, K, banks):
+    g = X.gen(M + N + K, "cuda")
+    ints = lambda n: torch.randint(-127, 128, (n, K), device="cuda", generator=g, dtype=torch.int32).to(torch.int8)
+    return (ints(M), torch.rand(M, device="cuda", generator=g) + 0.1, [ints(N) for _ in range(banks)],
+            [torch.rand(N, device="cuda", generator=g) * 1e-3 + 1e-5 for _ in range(banks)],
+            torch.randn(N, device="cuda", generator=g))
+
+
+@pytest.mark.parametrize("t,K", [(BF16, 4112), (BF16, 14336), (BF16, 16384), (F16, 5632), (F16, 14336), (F32, 2064),
+                                 (F32, 8192)])
+def test_long_float_token(dev, t, K):
+    """One token of more than 8 KB, quantized in the launch: four vectors a thread."""
+    _case(t="token", K=K, type=t)
+    g = X.gen(K, "cuda")
+    x = torch.randn(1, K, device="cuda", generator=g).to(t)
+    x[0, K - 1] = 9.0  # the row's largest value sits at its end
+    w = [torch.randint(-127, 128, (100, K), device="cuda", generator=g, dtype=torch.int32).to(torch.int8) for _ in range(2)]
+    s = [torch.rand(100, device="cuda", generator=g) * 1e-3 + 1e-5 for _ in range(2)]
+    q, sx = R.quantize(x)
+    ref, tol = R.matmul(q, sx, w[0], s[0])
+    y = mi_qmm.int8_matmul(x, w[0], s[0])
+    R.check(y, ref, tol(t), "y")
+    assert torch.equal(y, mi_qmm.int8_matmul(q, w[0], s[0], x_scales=sx, dtype=t))
+    assert torch.equal(y, mi_qmm.int8_matmul(_off(x, 1), w[0], s[0]))
+    h = mi_qmm.int8_gate_up_swiglu(x, w[0], s[0], w[1], s[1], save=True)
+    r = R.gate_up(q, sx, w[0], s[0], w[1], s[1])
+    for a, b, e in zip(h, r[:3], r[3:]):
+        R.check(a, b, e(t), "gate + up")
+    h2 = mi_qmm.int8_gate_up_swiglu(q, w[0], s[0], w[1], s[1], x_scales=sx, dtype=t, save=True)
+    assert all(torch.equal(a, b) for a, b in zip(h, h2))
+
+
+@pytest.mark.parametrize("N,K", [(8192, 64), (8197, 208), (14353, 48), (8200, 1040)])
+@pytest.mark.parametrize("M", [9, 16, 17, 32, 33, 48, 49, 64])
+def test_few_rows_of_wide_weights(dev, M, N, K):
+    """Two tiles of weights a wave."""
+    _case(t="wide", M=M, N=N, K=K)
+    q, sx, (w,), (s,), b = _codes(M, N, K, 1)
+    ref, tol = R.matmul(q, sx, w, s, b)
+    R.check(mi_qmm.int8_matmul(q, w, s, x_scales=sx, bias=b, dtype=F32), ref, tol(F32), "y")
+    ref, tol = R.matmul(q, sx, w, s)
+    R.check(mi_qmm.int8_matmul(q, w, s, x_scales=sx), ref, tol(BF16), "bf16")
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("M,N,K", [(1840, 578, 7429), (1843, 577, 7440)])
+def test_ranges_of_128_row_tiles(dev, M, N, K, t):
+    """All blocks in one round: the kernel that asks the L2 for its lines ahead."""
+    _case(t="ranges", M=M, N=N, K=K, type=t)
+    q, sx, (w,), (s,), b = _codes(M, N, K, 1)
+    ref, tol = R.matmul(q, sx, w, s, b.to(t))
+    R.check(mi_qmm.int8_matmul(q, w, s, x_scales=sx, bias=b.to(t), dtype=t), ref, tol(t), "y")
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("M,N,K", [(57, 853, 208), (64, 130, 1040), (49, 36, 77)])
+def test_gate_up_of_64_rows(dev, M, N, K, t):
+    _case(t="gate + up", M=M, N=N, K=K, type=t)
+    q, sx, w, s, _ = _codes(M, N, K, 2)
+    got = mi_qmm.int8_gate_up_swiglu(q, w[0], s[0], w[1], s[1], x_scales=sx, dtype=t, save=True)
+    r = R.gate_up(q, sx, w[0], s[0], w[1], s[1])
+    # half a step past a type's largest value a rounding is infinite (fp16: 65520)
+    top = float(torch.finfo(t).max)
+    border = top + 2.0 ** math.floor(math.log2(top)) * torch.finfo(t).eps / 2
+    for a, b, e in zip(got, r[:3], r[3:]):
+        over = b.abs() > border
+        assert ((b.abs() - border).abs() > e(t)).all()  # none lies next to the border
+        R.check(a, torch.where(over, b.sign() * torch.inf, b), e(t), "gate + up")
