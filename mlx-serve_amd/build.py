@@ -22,6 +22,8 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Wall",
          "-I", os.path.join(ROOT, "include"), "-I", HOST]
 TEST_SRC = os.path.join(ROOT, "tests", "cpp", "test_host.cpp")
 TEST_BIN = os.path.join(ROOT, "tests", "cpp", "_build", "test_host")
+PLAN_SRC = os.path.join(ROOT, "tests", "cpp", "int8_plan.cpp")
+PLAN_BIN = os.path.join(ROOT, "tests", "cpp", "_build", "int8_plan")
 
 
 def _stale(src, obj):
@@ -81,8 +83,15 @@ def build_host_tests(verbose=True):
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError("test_host build failed:\n" + r.stderr)
+    # which kernels the int8 calls take, for tests/test_int8_plans.py
+    cmd = [HIPCC, "-O2", "-std=c++17", "-x", "hip", "--offload-arch=gfx950", "-Xclang", "-target-feature", "-Xclang",
+           "-packed-fp32-ops", PLAN_SRC, "-I", os.path.join(HERE, "csrc"), "-L", OUT_DIR, "-lmi_qmm",
+           "-Wl,-rpath,$ORIGIN/../../../mlx-serve_amd/mi_qmm", "-o", PLAN_BIN]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("int8_plan build failed:\n" + r.stderr)
     if verbose:
-        print("built", TEST_BIN)
+        print("built", TEST_BIN, PLAN_BIN)
     return TEST_BIN
 
 

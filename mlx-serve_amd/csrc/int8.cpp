@@ -7,7 +7,15 @@
 
 namespace mi {
 int report_error(int code, const std::string& msg);  // sets mi_last_error() (api.cpp)
+
+// up to 16 rows the few-row kernel, up to 128 the one that should be faster
+void int8_forward_plan(Int8Params& P) {
+  P.ks = 1;
+  const double few = P.M <= kInt8FewRows ? int8_gemv_plan(P) : (P.nt = 0, 0.0);
+  if (P.M > 16 && int8_gemm_plan(P) < few) P.nt = 0;
+  if (P.nt) P.ks = 1;
 }
+}  // namespace mi
 
 namespace {
 
@@ -68,11 +76,7 @@ int64_t forward_need(mi::Int8Params& P, int64_t M, int64_t N, int64_t K, int x_d
   P.M = (int)M;
   P.N = (int)N;
   P.K = (int)up(K, 16);
-  P.ks = 1;
-  // up to 16 rows the few-row kernel, up to 128 the one that should be faster
-  const double few = M <= mi::kInt8FewRows ? mi::int8_gemv_plan(P) : (P.nt = 0, 0.0);
-  if (M > 16 && mi::int8_gemm_plan(P) < few) P.nt = 0;
-  if (P.nt) P.ks = 1;
+  mi::int8_forward_plan(P);
   return x_bytes(M, K, x_dtype) + sx_bytes(M, x_dtype) + P.banks * w_bytes(N, K) +
          (P.ks > 1 ? (int64_t)P.ks * P.banks * M * N * 4 : 0);
 }

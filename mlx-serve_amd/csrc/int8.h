@@ -82,6 +82,7 @@ struct Int8GradParams {
 
 hipError_t launch_int8_quantize(int8_t* q, float* s, const void* x, int64_t rows, int64_t K,
                                 int64_t ldq, int type, hipStream_t st);
+void int8_forward_plan(Int8Params& P);  // one of the two below, from the same (int8.cpp)
 double int8_gemv_plan(Int8Params& P);  // nt, from M, N, K and banks; returns estimated us
 bool int8_gemv_fuses(int64_t M, int64_t K, int type);
 hipError_t launch_int8_gemv(const Int8Params& P, hipStream_t s);
