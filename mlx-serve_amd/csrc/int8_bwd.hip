@@ -15,11 +15,11 @@
 // (subnormal, and exact).
 //
 // What bounds it: the matrix cores at the clock that the card's power allows. dx [4096,4096] of gate
-// + up [14336,4096] takes 686 us behind the gradient's pass, 1.40 PFLOP/s, where a bf16 library product
-// of 8192^3 runs at 1.41; MFMA instructions are busy 78% of the time. Without an alias scope of the
-// turned reads (read_tr8) it took 86 us more, stored straight from the products' layout
-// 13 us more. A dword of each line asked for in the L2 ahead of the DMA, which helps short rings in
-// int8_gemm.hip, made it 2 to 8% slower at every size and tile.
+// + up [14336,4096] takes 1360 us in two parts behind the gradient's pass (1440 where launches follow one another
+// at once), 1.41 PFLOP/s, where a bf16 library product of 8192^3 runs at 1.25 to 1.42; MFMA instructions are
+// busy 78% of the time. Measured with one part, 686 us: without an alias scope of the turned reads (read_tr8) 86
+// us more, stored straight from the products' layout 13 us more. A dword of each line asked for in the L2
+// ahead of the DMA, which helps short rings in int8_gemm.hip, made it 2 to 8% slower at every size and tile.
 #include <algorithm>
 #include <atomic>
 
@@ -309,15 +309,16 @@ hipError_t launch_tile(const Int8BwdParams& P, hipStream_t s) {
 
 }  // namespace
 
-// As int8_gemm_plan. Measured, us with the gradient's own pass, 256x256 / 128x256 / 128x128 tiles:
-//   dx [M,4096], sum of 4096   300 rows 39 / 32 / 33   1024 57 / 54 / 50    2048  85 /  75 /  84
-//   dx [M,14336], sum of 4096  300 rows 73 / 66 / 74   1024 111 / 139 / 150  2048 205 / 260 / 258
-//   dx [M,4096], gate + up sums of 14336   512 rows 142 / 158 / 172   4096 829 / 1016 / 1100
-// and 64x128, which lasts for few rows: dx [128,4096] of 4096 30 / 29 / 25 / 25.
+// As int8_gemm_plan. Measured, bf16, us with the gradient's own pass, 256x256 / 128x256 / 128x128 / 64x128 tiles:
+//   dx [M,4096], sum of 4096   128 rows 36 / 31 / 27 / 31   300 50 / 44 / 47 / 49   1024 82 / 84 / 94 / 113
+//                             2048 rows 134 / 138 / 155 / 209
+//   dx [M,14336], sum of 4096  300 rows 118 / 116 / 125 / 148   1024 191 / 247 / 275 / 359   2048 376 / 486 / 497 / 688
+//   dx [M,4096], gate + up sums of 14336   512 rows 231 / 261 / 291 / 389   4096 1535 / 1992 / 2207 / 3005
+// and as planned 28, 44, 84, 138; 117, 191, 375; 228, 1529. 64x128 tiles last for fewer rows and shorter sums.
 void int8_bwd_plan(Int8BwdParams& P) {
   const int steps = P.banks * P.terms * (P.np / kBN_);
   constexpr TileCost kTiles[] = {
-      {256, 256, 1.47, 0.0, 8.0}, {128, 256, 0.92, 0.0, 4.0}, {128, 128, 0.6, 1.07, 3.0}, {64, 128, 0.5, 0.8, 3.0}};
+      {256, 256, 1.47, 0.0, 8.0}, {128, 256, 0.92, 0.0, 4.0}, {128, 128, 0.64, 1.07, 3.0}, {64, 128, 0.5, 0.8, 3.0}};
   double best = 1e30;
   for (const TileCost& t : kTiles) {
     const int64_t tiles = (int64_t)((P.M + t.bm - 1) / t.bm) * ((P.K + t.bn - 1) / t.bn);
