@@ -292,9 +292,10 @@ int mi_gather_qmv_down_reduce(void* y, const void* act, const uint32_t* w_down,
  * this one has run; its size comes from the two functions below (host only; may be 0, then
  * NULL will do; -1 for sizes or types out of range). It holds the quantized tokens, scaled gradients
  * or partial sums, and, where K is no multiple of 16, a copy of the weights in rows that are: lay such
- * weights out with zeros up to 16 for speed. A missing or short one is MI_ERR_WORKSPACE. These calls allocate nothing and keep nothing, so they can be captured into
- * graphs as they are, and run at the same time on several streams with a workspace each. Tensors
- * and stream belong to the current device.
+ * weights out with zeros up to 16 for speed. A missing or short one is MI_ERR_WORKSPACE.
+ *
+ * These calls allocate nothing and keep nothing, so they can be captured into graphs as they are, and run
+ * at the same time on several streams with a workspace each. Tensors and stream belong to the current device.
  * Outputs must not overlap inputs. Empty outputs (M = 0, ...) are no-ops; a sum over nothing
  * (K = 0 forward, N = 0 backward) is MI_ERR_INVALID. K over 131071 forward, where the int32 sums
  * of the products could overflow, is MI_ERR_UNSUPPORTED. */
@@ -317,9 +318,9 @@ int mi_int8_matmul(void* y, const void* x, const float* x_scales, const int8_t* 
                    int x_dtype, int y_dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* y = silu(g) * u with g and u the products of x with w_gate and w_up (as mi_int8_matmul),
- * silu(g) = g / (1 + e^-g) in fp32 (where y is bfloat16 or float16 the exponential is good to
- * (5 + 1.25 |g|) 2^-24, below their own last bit), one rounding. gate and up: both NULL, or [M, N] in y's type
- * for g and u, each rounded once, as the backward pass takes them. */
+ * silu(g) = g s, s = 1 / (1 + e^-g), in fp32, one rounding. (Where y is bfloat16 or float16, s is good to
+ * (5 + 1.25 |g|) 2^-24 of itself, less than their last bit, and 0 below 2^-126.) gate and up: both NULL,
+ * or [M, N] in y's type for g and u, each rounded once, as the backward pass takes them. */
 int mi_int8_gate_up_swiglu(void* y, void* gate, void* up, const void* x, const float* x_scales,
                            const int8_t* w_gate, const float* s_gate, const int8_t* w_up,
                            const float* s_up, int64_t M, int64_t N, int64_t K, int x_dtype,
@@ -336,7 +337,7 @@ int mi_int8_matmul_backward(void* dx, const void* dy, const int8_t* w, const flo
                             int64_t workspace_bytes, void* stream);
 
 /* The gradients of mi_int8_gate_up_swiglu: with s = 1 / (1 + e^-g),
- *   dgate = dy * u * s * (1 + g (1 - s)),   dup = dy * g * s   (fp32, s as in the forward call, one rounding each)
+ *   dgate = dy * u * s * (1 + g (1 - s)),   dup = dy * g * s   (fp32, s as above, one rounding each)
  *   dx[m,k] = sum_n dgate[m,n] s_gate[n] w_gate[n,k] + dup[m,n] s_up[n] w_up[n,k]
  * from gate and up as the forward call gave them; dx is formed from dgate and dup before their
  * rounding, otherwise as mi_int8_matmul_backward. dgate and dup ([M, N], both or neither NULL)

@@ -13,11 +13,13 @@
 // exact vmcnt.
 //
 // What bounds it: large products the matrix cores and the DMA beside them at the clock that the card's
-// power allows: 8192 x 4096 x 14336 in 361 us, 2.66 POPS (a library product of the same codes: 402 to
-// 459 us, by their values); MFMA instructions are busy 67% of the time. 64-byte steps in a ring of
-// five stages took 444 us, weights straight into registers 455, four waves of 128 x 128 each (a third
+// power allows: 8192 x 4096 x 14336 in 360 to 370 us among other calls, 2.6 POPS (395 to 415 where launches
+// follow one another at once), MFMA instructions busy 66% of the time. In turn with it and on the same codes
+// a library product to int32, without the scales, took 382 to 391. 64-byte steps in a ring of five stages took
+// 444 us against 361 to 377, weights straight into registers 455, four waves of 128 x 128 each (a third
 // less read from LDS, one wave a SIMD) 444, 32 x 32 x 32 instructions 410. Up to 256 rows or so the weights
-// from HBM bound it: gate + up [14336,4096], 48 rows, 25.9 us (4.5 TB/s). Two things keep them coming:
+// from HBM bound it: gate + up [14336,4096], 48 rows, 25.9 us (4.5 TB/s; graphs over more weights than the
+// last-level cache holds). Two things keep them coming:
 // - Rows of a power-of-two pitch meet in the same memory channels. Up to 256 rows a column tile starts
 //   3 steps further along K than the one before it and wraps round (int32 sums, exact in any
 //   order): 25.9 us against 30.6 there. With more rows tiles share lines in the L2 by reading them

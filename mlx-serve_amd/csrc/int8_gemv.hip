@@ -1,4 +1,5 @@
-// Int8 products of few rows (up to 128): decode, and short prompts through small matrices. The weights are read once, so their bytes bound it.
+// Int8 products of few rows (up to 128): decode, and short prompts through small matrices. The weights are
+// read once, so their bytes bound it.
 //
 // Block: WK waves that share 16 NT rows of w (of both banks, with two) and split K between them;
 // a wave streams its part of those rows straight into registers (one instruction reads 16 rows x 64
@@ -11,8 +12,8 @@
 // One float token (FUSE): each block quantizes it by itself, into LDS, while its first weights are on
 // their way: it is a few KB, and a launch of its own costs more (2 us and the gap before it).
 //
-// Measured in graphs, us: [14336,4096] 1 token 15.7, 2 rows 14.6 (4.0 TB/s), 8 rows 17.0;
-// [4096,14336] 14.5, 13.4 and 15.7; [4096,4096] 6.2, 5.9 and 6.4; gate + up [14336,4096] 1 token 27.5
+// Measured in graphs over more weights than the last-level cache (256 MB) holds, us: [14336,4096] 1 token
+// 15.7, 2 rows 14.6 (4.0 TB/s), 8 rows 17.0; [4096,14336] 14.5, 13.4 and 15.7; [4096,4096] 6.2, 5.9 and 6.4; gate + up [14336,4096] 1 token 27.5
 // (4.3 TB/s), 16 rows 29. Above 16 rows the reads of x from the L2 count: [4096,4096] 16 rows 7.4,
 // 64 rows 13.2. (Two chunks that share a line, 16 of each 32 bytes for either, so that the first load
 // asks for the whole line, took 0.2 us off one token of [4096,4096] and put up to 1.3 us on 8 rows;

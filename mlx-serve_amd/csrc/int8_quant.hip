@@ -159,8 +159,8 @@ hipError_t launch_type(int8_t* q, float* s, const void* x, int64_t rows, int64_t
 // subnormal, the matrix instructions cut the others off at 2^-51). A row with an infinity or a NaN is taken as
 // it is.
 //
-// Memory-bound (three reads, four writes of [M, N] with both outputs); a row is held in
-// registers between its maximum and the parts. Measured: [4096,14336] bf16 gate + up 160 us, 5.1 TB/s.
+// Memory-bound (three reads, six writes of [M, N] with both outputs); a row is held in
+// registers between its maximum and the parts. Measured: [4096,14336] bf16 gate + up 205 us, 5.2 TB/s.
 
 // power of two for a row whose largest finite magnitude has these bits, and its reciprocal
 MI_DEV void row_power(uint32_t maxbits, float* scale, float* inv) {

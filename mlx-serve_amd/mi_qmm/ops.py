@@ -521,8 +521,9 @@ def int8_matmul(x, w, w_scales, x_scales=None, bias=None, dtype=None):
 
 
 def int8_gate_up_swiglu(x, wg, sg, wu, su, x_scales=None, dtype=None, save=False):
-    """silu(x @ wg.T) * (x @ wu.T) in one launch, operands as int8_matmul. save=True returns
-    (y, gate, up), the two projections for int8_gate_up_swiglu_backward."""
+    """silu(x @ wg.T) * (x @ wu.T) by one kernel (float x of more than one row is quantized before it),
+    operands as int8_matmul. save=True returns (y, gate, up), the two projections for
+    int8_gate_up_swiglu_backward."""
     if wg.dim() != 2:
         _bad("weights must be int8 [N, K]")
     N, K = wg.shape
